@@ -95,6 +95,14 @@ int encode_tmap_2d_u8_sw64(CUtensorMap* map, const void* base, uint64_t inner, u
   return encode(map, base, 2, dims, strides, box, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
+int encode_tmap_2d_u8(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t row_stride_bytes,
+                      uint32_t box_inner, uint32_t box_outer) {
+  const cuuint64_t dims[2] = {inner, outer};
+  const cuuint64_t strides[1] = {row_stride_bytes};
+  const cuuint32_t box[2] = {box_inner, box_outer};
+  return encode(map, base, 2, dims, strides, box, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
 int encode_tmap_3d_i8(CUtensorMap* map, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t stride1,
                       uint64_t stride2, uint32_t box0, uint32_t box1) {
   const cuuint64_t dims[3] = {d0, d1, d2};
@@ -230,12 +238,13 @@ extern "C" int fni8_device_status(int* code_out) {
   if (code_out == nullptr) return fail(FNI8_ERR_INVALID, "null code_out");
   cudaError_t e = cudaDeviceSynchronize();
   if (e != cudaSuccess) return cuda_status(e, "cudaDeviceSynchronize");
-  int codes[5] = {0, 0, 0, 0, 0};
+  int codes[6] = {0, 0, 0, 0, 0, 0};
   if (int s = tile_status_read_and_clear(&codes[0])) return s;
   if (int s = stream_status_read_and_clear(&codes[1])) return s;
   if (int s = splitk_status_read_and_clear(&codes[2])) return s;
   if (int s = w4a8_status_read_and_clear(&codes[3])) return s;
   if (int s = ep_status_read_and_clear(&codes[4])) return s;
+  if (int s = fp4_status_read_and_clear(&codes[5])) return s;
   *code_out = 0;
   for (int v : codes)
     if (*code_out == 0) *code_out = v;

@@ -1,0 +1,118 @@
+// 4-bit floating point (e2m1) with block scales: the layout shared by the row kernels
+// (fp4.cu) and the block-scaled GEMMs (gemm_fp4.cu, gemm_fp4_splitk.cu).
+//
+//   FNI8_MXFP4  one e8m0 scale (a power of two) for every 32 values
+//   FNI8_NVFP4  one e4m3 scale for every 16 values, and one fp32 scale for each row
+//
+// Codes: two to a byte, the even element in the low half, rows of Kp / 2 bytes with
+// Kp = K rounded up to 32 (zero codes behind K). Scales: tiles of 128 rows x 4 scales, 512
+// bytes each, tile (r / 128, s / 4) at index (r / 128) * ceil(S / 4) + s / 4, where row r
+// and scale s are at byte (r % 32) * 16 + (r % 128 / 32) * 4 + s % 4: the order in which
+// tcgen05.cp.32x128b.warpx4 brings a tile into tensor memory, four scales of a row in one
+// 32-bit cell. Scales behind K are zero, so the padded part of a tile adds nothing.
+#pragma once
+#include "fni8_common.cuh"
+
+namespace fni8b {
+namespace fp4 {
+
+template <int FMT>
+struct Fmt;
+template <>
+struct Fmt<FNI8_MXFP4> {
+  static constexpr int kBlock = 32;
+  static constexpr int kStageTiles = 2;  // scale tiles of a 256-value (128-byte) stage
+};
+template <>
+struct Fmt<FNI8_NVFP4> {
+  static constexpr int kBlock = 16;
+  static constexpr int kStageTiles = 4;
+};
+
+__host__ __device__ __forceinline__ int64_t padded_k(int64_t K) { return (K + 31) / 32 * 32; }
+// scale tiles along K
+__host__ __device__ __forceinline__ int64_t k_tiles(int fmt, int64_t K) {
+  return fmt == FNI8_MXFP4 ? (K + 127) / 128 : (K + 63) / 64;
+}
+__host__ __device__ __forceinline__ int64_t row_tiles(int64_t M) { return (M + 127) / 128; }
+// byte of row r within its column of tiles (add tile * 512 and s % 4)
+__device__ __forceinline__ int row_byte(int r) { return (r & 31) * 16 + ((r & 127) >> 5) * 4; }
+
+// Instruction descriptor of tcgen05.mma kind::mxf4 / kind::mxf4nvf4: A = B = e2m1, both
+// K-major, dense, K = 64, shape M x N; sf_id: which two of a cell's four scales (0 or 2)
+// an mxfp4 step takes (nvfp4 takes all four, sf_id 0).
+__host__ __device__ constexpr uint32_t idesc_fp4(int fmt, int M, int N, int sf_id) {
+  return (static_cast<uint32_t>(sf_id) << 4)                      // B scales
+         | (1u << 7) | (1u << 10)                                 // A, B: e2m1
+         | (static_cast<uint32_t>(N >> 3) << 17)                  // N / 8
+         | ((fmt == FNI8_MXFP4 ? 1u : 0u) << 23)                  // scales: e8m0 (1) or e4m3 (0)
+         | (static_cast<uint32_t>(M >> 7) << 27)                  // M / 128
+         | (static_cast<uint32_t>(sf_id) << 29);                  // A scales
+}
+
+// Shared-memory descriptor of one 512-byte scale tile for tcgen05.cp: 32 rows of 16 bytes,
+// no swizzle, 128 bytes from one group of 8 rows to the next.
+__device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
+  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(128u >> 4) << 32) |
+         (static_cast<uint64_t>(1u) << 46);
+}
+
+template <bool PAIR>
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
+  if constexpr (PAIR)
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+// D[tmem] (+)= (A * SFA)[smem] * (B * SFB)[smem]^T over 64 values of K, issued by one thread.
+#define FNI8_MMA_FP4(GROUP, KIND, VEC)                                                             \
+  asm volatile(                                                                                    \
+      "{\n\t.reg .pred p;\n\t"                                                                     \
+      "setp.ne.b32 p, %6, 0;\n\t"                                                                  \
+      "tcgen05.mma.cta_group::" GROUP ".kind::" KIND ".block_scale.scale_vec::" VEC                \
+      " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),                                           \
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)                      \
+      : "memory")
+template <int FMT, bool PAIR>
+__device__ __forceinline__ void umma_fp4(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa,
+                                         uint32_t sfb, uint32_t accumulate) {
+  if constexpr (FMT == FNI8_MXFP4) {
+    if constexpr (PAIR) FNI8_MMA_FP4("2", "mxf4", "2X");
+    else FNI8_MMA_FP4("1", "mxf4", "2X");
+  } else {
+    if constexpr (PAIR) FNI8_MMA_FP4("2", "mxf4nvf4", "4X");
+    else FNI8_MMA_FP4("1", "mxf4nvf4", "4X");
+  }
+}
+#undef FNI8_MMA_FP4
+
+// The 256-value stage's MMAs: `steps` (1 to 4) of 64 values each. sa, sb: the operands'
+// stage (128-byte swizzle), ta, tb: the tensor-memory columns of their scales.
+template <int FMT, bool PAIR, int M, int N>
+__device__ __forceinline__ void stage_mmas(uint32_t d, const void* sa, const void* sb, uint32_t ta, uint32_t tb,
+                                           int steps, bool first) {
+  constexpr int kBCols = (N + 127) / 128 * 4;  // columns of one tile column of B's scales
+  const uint64_t adesc = sw128_kmajor_desc(smem_u32(sa)), bdesc = sw128_kmajor_desc(smem_u32(sb));
+#pragma unroll
+  for (int kk = 0; kk < 4; ++kk) {
+    if (kk < steps) {
+      const int tile = FMT == FNI8_MXFP4 ? kk >> 1 : kk;
+      const uint32_t idesc = idesc_fp4(FMT, M, N, FMT == FNI8_MXFP4 ? (kk & 1) * 2 : 0);
+      umma_fp4<FMT, PAIR>(d, adesc + static_cast<uint64_t>(kk * 2), bdesc + static_cast<uint64_t>(kk * 2), idesc,
+                          ta + static_cast<uint32_t>(tile * 4), tb + static_cast<uint32_t>(tile * kBCols),
+                          (kk != 0 || !first) ? 1u : 0u);
+    }
+  }
+}
+
+}  // namespace fp4
+}  // namespace fni8b
+
+namespace fni8h {
+// The scale tiles as a 2-D map of 128-byte rows (four to a tile); a box is `tiles` of them.
+inline int encode_scale_map(CUtensorMap* map, const uint8_t* sf, int fmt, int64_t M, int64_t K, int tiles) {
+  const int64_t rows = fni8b::fp4::row_tiles(M) * fni8b::fp4::k_tiles(fmt, K) * 4;
+  return encode_tmap_2d_u8(map, sf, 128, (uint64_t)rows, 128, 128, (uint32_t)(tiles * 4));
+}
+}  // namespace fni8h

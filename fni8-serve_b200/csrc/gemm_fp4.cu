@@ -1,0 +1,508 @@
+// GEMM of 4-bit floating point operands on the block-scaled tensor core (sm_100a).
+//
+//   out[m, n] = dtype((sum_k a[m,k] sa[m,k/g] w[n,k] sw[n,k/g]) * ra[m] * rw[n] (+ bias[n]))
+//
+// a, w: e2m1 codes, sa, sw: their block scales (fp4_common.cuh), ra, rw: the row scales of
+// nvfp4. tcgen05.mma kind::mxf4 / kind::mxf4nvf4 applies the block scales, so the fp32
+// accumulator holds the finished sum and the epilogue only multiplies by the row scales.
+//
+// Structure of the int8 tile kernel (gemm_tile.cu): one persistent CTA per SM, a TMA warp,
+// an MMA warp, eight epilogue warps. A stage is 128 bytes of K (256 values) of 128 rows of a
+// and BN rows of w with the 128-byte swizzle, plus their scale tiles as they lie in memory
+// (512 bytes each, no swizzle); the MMA thread copies the scale tiles into tensor memory
+// with tcgen05.cp before the stage's four MMAs. Copies and MMAs of one thread execute in
+// order, so a stage's scales need no wait; two sets of tensor-memory columns alternate.
+#include "fp4_common.cuh"
+#include "gemm_internal.h"
+
+namespace fni8b {
+namespace fp4 {
+
+constexpr int BM = 128;
+constexpr int BK = 128;  // bytes of K per stage: 256 values
+constexpr int kEpiWarps = 8;
+constexpr int kEpiThreads = 32 * kEpiWarps;
+constexpr int kTileThreads = 64 + kEpiThreads;
+constexpr int kBand = 16;  // m-tiles per band of the tile order: a wave reuses its rows and columns from L2
+
+static __device__ int g_status;
+
+enum : int { kCodeProducer = 0x701, kCodeMma = 0x702, kCodeEpilogue = 0x703, kCodeDrain = 0x704 };
+
+struct Epi {
+  const float* a_rs;  // [M] or null (mxfp4)
+  const float* w_rs;  // [N] or null
+  const void* bias;   // [N] or null
+  void* out;          // [M, N]
+  int bf16;
+  int tma_store;  // rows 16-byte aligned: slabs leave by TMA
+};
+
+template <int FMT, int BN, bool PAIR>
+struct Cfg {
+  static constexpr int BMT = PAIR ? 2 * BM : BM;  // rows of a tile
+  static constexpr int BNL = PAIR ? BN / 2 : BN;  // weight rows this CTA loads per stage
+  static constexpr int TILES = Fmt<FMT>::kStageTiles;
+  static constexpr int A_BYTES = BM * BK;
+  static constexpr int B_BYTES = BNL * BK;
+  static constexpr int SFA_BYTES = TILES * 512;
+  static constexpr int SFB_BYTES = BN / 128 * TILES * 512;  // of all BN columns, in both CTAs of a pair
+  static constexpr int STAGE = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
+  static constexpr int STG_BUF = 32 * 32 * 2;  // one output slab of an epilogue warp
+  static constexpr int FIXED = 1024 + 1024 + kEpiWarps * STG_BUF + 2 * BN * 4;
+  static constexpr int STAGES = (227 * 1024 - FIXED) / STAGE;
+  static constexpr int STG_OFF = STAGES * STAGE + 1024;  // barriers in between; 1024-aligned
+  static constexpr int SMEM = FIXED + STAGES * STAGE;
+  // accumulators in columns [0, 256), then two sets of scale columns
+  static constexpr int NACC = 256 / BN;
+  static constexpr int SFA_COLS = TILES * 4;
+  static constexpr int SF_COLS = SFA_COLS + BN / 128 * TILES * 4;
+  static_assert(256 + 2 * SF_COLS <= 512, "tensor memory");
+  static_assert(STAGES >= 3 && STAGES <= 8, "ring");
+};
+
+template <int BMT>
+__device__ __forceinline__ void tile_at(int t, int m_tiles, int n_tiles, int& m_blk, int& n_blk) {
+  const int band_tiles = kBand * n_tiles;
+  const int b = t / band_tiles;
+  const int first = b * kBand;
+  const int gm = min(kBand, m_tiles - first);
+  const int local = t - b * band_tiles;
+  m_blk = first + local % gm;
+  n_blk = local / gm;
+}
+
+// 32 accumulators of one row, scaled, biased and rounded: four 16-byte pieces.
+template <typename T, int FMT>
+__device__ __forceinline__ void finish_chunk(const uint32_t (&r)[32], float ra, const float* rw, const float* bs,
+                                             bool has_bias, uint4 (&o)[4]) {
+#pragma unroll
+  for (int j8 = 0; j8 < 4; ++j8) {
+    T* oo = reinterpret_cast<T*>(&o[j8]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int c = j8 * 8 + j;
+      float v = __uint_as_float(r[c]);
+      if constexpr (FMT == FNI8_NVFP4) v = __fmul_rn(__fmul_rn(v, ra), rw[c]);
+      if (has_bias) v = __fadd_rn(v, bs[c]);
+      oo[j] = from_f32<T>(v);
+    }
+  }
+}
+
+// A warp's 32 x 32 slab (lane = row) through its staging buffer: one TMA store, or, where
+// the rows are not 16-byte aligned, 64 contiguous bytes of a row per store instruction.
+__device__ __forceinline__ void store_slab(uint8_t* buf, const uint4 (&o)[4], int lane, const CUtensorMap* map,
+                                           bool tma, uint16_t* out, int n0, int N, int64_t row0, int rows) {
+  if (tma && lane == 0) bulk_wait_group_read<0>();
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    *reinterpret_cast<uint4*>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = o[j];
+  if (tma) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_2d(map, buf, n0, static_cast<int>(row0));
+      bulk_commit_group();
+    }
+  } else {
+    __syncwarp();
+    const int n = n0 + lane;
+    for (int r = 0; r < rows; ++r) {
+      const uint16_t v =
+          *reinterpret_cast<const uint16_t*>(buf + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
+      if (n < N) out[(row0 + r) * N + n] = v;
+    }
+    __syncwarp();
+  }
+}
+
+template <int FMT, int BN, bool PAIR>
+__global__ void __launch_bounds__(kTileThreads, 1)
+    fp4_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                    const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
+                    const __grid_constant__ CUtensorMap tmOut, Epi epi, int M, int N, int Kp, int ktiles) {
+  using C = Cfg<FMT, BN, PAIR>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE);
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* tfull = empty + C::STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* drain = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint8_t* stg = smem + C::STG_OFF;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t half = PAIR ? (cluster_ctarank() & 1u) : 0u;
+  const int t0 = PAIR ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
+  const int tstep = PAIR ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], PAIR ? 2 * kEpiWarps : kEpiWarps);
+    }
+    mbar_init(drain, 1);
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    if constexpr (PAIR) {
+      tmem_alloc_pair(tmem_slot, 512);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, 512);
+      tmem_relinquish();
+    }
+    tc_fence_before();
+  }
+  // the producer starts its weight loads before it waits for the quantiser
+  if (!(warp == 0 && lane == 0)) pdl_wait();
+  const int n_tiles = (N + BN - 1) / BN;
+  const int m_tiles = (M + C::BMT - 1) / C::BMT;
+  const int total = m_tiles * n_tiles;
+  const int kb = (Kp + 255) / 256;
+  if constexpr (PAIR) cluster_sync_all();
+  else __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      tma_prefetch_desc(&tmA);
+      tma_prefetch_desc(&tmB);
+      tma_prefetch_desc(&tmSA);
+      tma_prefetch_desc(&tmSB);
+      constexpr uint32_t kTx = PAIR ? 2 * C::STAGE : C::STAGE;
+      auto load = [&](const CUtensorMap* map, int s, int off, int cx, int cy) {
+        uint8_t* dst = smem + s * C::STAGE + off;
+        if constexpr (PAIR) tma_load_2d_pair(map, mapa_shared(smem_u32(&full[s]), 0), dst, cx, cy);
+        else tma_load_2d(map, &full[s], dst, cx, cy);
+      };
+      auto load_a = [&](int s, int m_blk, int k) {
+        const int rt = PAIR ? 2 * m_blk + static_cast<int>(half) : m_blk;  // this CTA's 128 rows
+        load(&tmA, s, 0, k * BK, rt * BM);
+        load(&tmSA, s, C::A_BYTES + C::B_BYTES, 0, (rt * ktiles + k * C::TILES) * 4);
+      };
+      auto load_b = [&](int s, int n_blk, int k) {
+        load(&tmB, s, C::A_BYTES, k * BK, n_blk * BN + static_cast<int>(half) * C::BNL);
+#pragma unroll
+        for (int i = 0; i < BN / 128; ++i)
+          load(&tmSB, s, C::A_BYTES + C::B_BYTES + C::SFA_BYTES + i * C::TILES * 512, 0,
+               ((n_blk * (BN / 128) + i) * ktiles + k * C::TILES) * 4);
+      };
+      int stage = 0, issued = 0, t = t0, k = 0, mb = 0, nb = 0;
+      uint32_t ph = 0, armed = 0;
+      if (t < total) tile_at<C::BMT>(t, m_tiles, n_tiles, mb, nb);
+      auto advance = [&]() {
+        if (++k == kb) {
+          k = 0;
+          t += tstep;
+          if (t < total) tile_at<C::BMT>(t, m_tiles, n_tiles, mb, nb);
+        }
+      };
+      int pre_m[C::STAGES], pre_k[C::STAGES];
+      int pre = 0;
+      for (; pre < C::STAGES && t < total; ++pre, advance()) {
+        if (half == 0) mbar_arrive_expect_tx(&full[pre], kTx);
+        load_b(pre, nb, k);
+        pre_m[pre] = mb;
+        pre_k[pre] = k;
+      }
+      pdl_wait();
+      for (int i = 0; i < pre; ++i) load_a(i, pre_m[i], pre_k[i]);
+      issued = pre;
+      stage = pre % C::STAGES;
+      ph = pre == C::STAGES ? 1u : 0u;
+      for (; t < total; advance()) {
+        if (!mbar_wait(&empty[stage], ph ^ 1u, &g_status, kCodeProducer)) break;
+        if (half == 0) mbar_arrive_expect_tx(&full[stage], kTx);
+        load_a(stage, mb, k);
+        load_b(stage, nb, k);
+        armed = (armed & ~(1u << stage)) | (ph << stage);
+        ++issued;
+        if (++stage == C::STAGES) {
+          stage = 0;
+          ph ^= 1u;
+        }
+      }
+      pdl_launch_dependents();
+      // every load lands before the CTA may exit (the odd CTA of a pair sees its loads land
+      // through the release of the stage)
+      uint64_t* done = half == 0 ? full : empty;
+      const int pending = issued < C::STAGES ? issued : C::STAGES;
+      for (int i = 0; i < pending; ++i) {
+        const int s = (stage - 1 - i + 2 * C::STAGES) % C::STAGES;
+        mbar_wait(&done[s], (armed >> s) & 1u, &g_status, kCodeDrain);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0 && half == 0) {
+      int stage = 0, acc = 0, set = 0;
+      uint32_t ph = 0, aph = 0;
+      bool ok = true;
+      for (int t = t0; t < total && ok; t += tstep) {
+        if (!mbar_wait(&tempty[acc], aph ^ 1u, &g_status, kCodeMma)) break;
+        tc_fence_after();
+        const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
+        for (int k = 0; k < kb; ++k) {
+          if (!mbar_wait(&full[stage], ph, &g_status, kCodeMma)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint8_t* sa = smem + stage * C::STAGE;
+          const uint8_t* sfa = sa + C::A_BYTES + C::B_BYTES;
+          const uint32_t ta = tmem_base + 256u + static_cast<uint32_t>(set * C::SF_COLS);
+          const uint32_t tb = ta + C::SFA_COLS;
+#pragma unroll
+          for (int i = 0; i < C::TILES; ++i) {
+            copy_scales<PAIR>(ta + i * 4, scale_desc(smem_u32(sfa + i * 512)));
+#pragma unroll
+            for (int j = 0; j < BN / 128; ++j)
+              copy_scales<PAIR>(tb + (i * (BN / 128) + j) * 4,
+                                scale_desc(smem_u32(sfa + C::SFA_BYTES + (j * C::TILES + i) * 512)));
+          }
+          const int steps = min(4, (Kp - k * 256 + 63) / 64);
+          stage_mmas<FMT, PAIR, C::BMT, BN>(d, sa, sa + C::A_BYTES, ta, tb, steps, k == 0);
+          if constexpr (PAIR) umma_commit_pair_to(&empty[stage], 3);
+          else umma_commit(&empty[stage]);
+          set ^= 1;
+          if (++stage == C::STAGES) {
+            stage = 0;
+            ph ^= 1u;
+          }
+        }
+        if (!ok) break;
+        if constexpr (PAIR) umma_commit_pair_to(&tfull[acc], 3);
+        else umma_commit(&tfull[acc]);
+        if (++acc == C::NACC) {
+          acc = 0;
+          aph ^= 1u;
+        }
+      }
+      if constexpr (PAIR) umma_commit_pair(drain);
+      else umma_commit(drain);
+      mbar_wait(drain, 0, &g_status, kCodeDrain);
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ epilogue
+    // Warp w reads the TMEM lanes [32 q, 32 q + 32), q = w % 4, and half of the columns. All
+    // of its outputs are formed in registers first, which frees the accumulator for the next
+    // tile before they are stored.
+    const int q = warp & 3, ew = warp - 2, et = threadIdx.x - 64;
+    const int c_beg = (ew >> 2) * (BN / 2);
+    float* s_rw = reinterpret_cast<float*>(stg + kEpiWarps * C::STG_BUF);
+    float* s_bias = s_rw + BN;
+    int acc = 0;
+    uint32_t aph = 0;
+    if (epi.tma_store && lane == 0) tma_prefetch_desc(&tmOut);
+    for (int t = t0; t < total; t += tstep) {
+      int mb, nb;
+      tile_at<C::BMT>(t, m_tiles, n_tiles, mb, nb);
+      const int64_t row0 = static_cast<int64_t>(mb) * C::BMT + static_cast<int>(half) * BM + q * 32;
+      const int64_t row = row0 + lane;
+      const int rows = static_cast<int>(M - row0 < 32 ? (M > row0 ? M - row0 : 0) : 32);
+      float ra = 1.0f, rw = 1.0f, bs = 0.0f;
+      if (et < BN && nb * BN + et < N) {
+        const int n = nb * BN + et;
+        if constexpr (FMT == FNI8_NVFP4) rw = __ldg(epi.w_rs + n);
+        if (epi.bias != nullptr)
+          bs = epi.bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(epi.bias)[n])
+                        : __half2float(static_cast<const __half*>(epi.bias)[n]);
+      }
+      if constexpr (FMT == FNI8_NVFP4)
+        if (row < M) ra = __ldg(epi.a_rs + row);
+      int ok = 0;
+      if (lane == 0) ok = mbar_wait(&tfull[acc], aph, &g_status, kCodeEpilogue) ? 1 : 0;
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!named_bar_and(2, kEpiThreads, ok)) break;  // also: the previous tile's scales are read
+      tc_fence_after();
+      if (et < BN) {
+        s_rw[et] = rw;
+        s_bias[et] = bs;
+      }
+      named_bar_sync(2, kEpiThreads);
+      const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BN + c_beg);
+      constexpr int kChunks = BN / 64;
+      uint4 o[kChunks][4];
+      uint32_t r[32];
+      tmem_ld32(tb, r);
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        tmem_ld_wait();
+        tmem_regs_ready(r);
+        const float* w = s_rw + c_beg + c * 32;
+        const float* b = s_bias + c_beg + c * 32;
+        if (epi.bf16) finish_chunk<__nv_bfloat16, FMT>(r, ra, w, b, epi.bias != nullptr, o[c]);
+        else finish_chunk<__half, FMT>(r, ra, w, b, epi.bias != nullptr, o[c]);
+        if (c + 1 < kChunks) tmem_ld32(tb + (c + 1) * 32, r);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (half == 0) mbar_arrive(&tempty[acc]);
+        else mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[acc]), 0));
+      }
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        const int n0 = nb * BN + c_beg + c * 32;
+        if (rows > 0 && n0 < N)
+          store_slab(stg + ew * C::STG_BUF, o[c], lane, &tmOut, epi.tma_store != 0, static_cast<uint16_t*>(epi.out), n0,
+                     N, row0, rows);
+      }
+      if (++acc == C::NACC) {
+        acc = 0;
+        aph ^= 1u;
+      }
+    }
+    if (epi.tma_store && lane == 0) bulk_wait_group<0>();
+    __syncwarp();
+  }
+
+  if constexpr (PAIR) cluster_sync_all();
+  else __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (PAIR) tmem_dealloc_pair(tmem_base, 512);
+    else tmem_dealloc(tmem_base, 512);
+  }
+}
+
+}  // namespace fp4
+}  // namespace fni8b
+
+namespace fni8h {
+
+using namespace fni8b;
+
+int fp4_status_read_and_clear(int* code) {
+  int v = 0, z = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, fp4::g_status, sizeof(int));
+  if (e != cudaSuccess) return cuda_status(e, "read fp4 watchdog");
+  e = cudaMemcpyToSymbol(fp4::g_status, &z, sizeof(int));
+  if (e != cudaSuccess) return cuda_status(e, "clear fp4 watchdog");
+  *code = v;
+  return FNI8_OK;
+}
+
+namespace {
+
+template <int FMT, int BN, bool PAIR>
+int launch_tile(const Fp4Gemm& g, cudaStream_t st) {
+  using C = fp4::Cfg<FMT, BN, PAIR>;
+  auto kern = fp4::fp4_tile_kernel<FMT, BN, PAIR>;
+  static std::atomic<bool> configured[kMaxDevices] = {};
+  const int dev = current_device();
+  if (dev < 0 || dev >= kMaxDevices) return fail(FNI8_ERR_CUDA, "no current CUDA device");
+  if (!configured[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(fp4 gemm)");
+    configured[dev] = true;
+  }
+  const uint64_t row = (uint64_t)fp4::padded_k(g.K) / 2;
+  CUtensorMap ta, tb, tsa, tsb, to = {};
+  if (int s = encode_tmap_2d_i8(&ta, g.a, row, (uint64_t)g.M, row, 128, 128)) return s;
+  if (int s = encode_tmap_2d_i8(&tb, g.w, row, (uint64_t)g.N, row, 128, (uint32_t)C::BNL)) return s;
+  if (int s = encode_scale_map(&tsa, g.a_sf, FMT, g.M, g.K, C::TILES)) return s;
+  if (int s = encode_scale_map(&tsb, g.w_sf, FMT, g.N, g.K, C::TILES)) return s;
+  fp4::Epi epi{g.a_rs, g.w_rs, g.bias, g.out, g.bf16 ? 1 : 0, 0};
+  if (g.N % 8 == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15u) == 0) {
+    if (int s = encode_tmap_2d_16_sw(&to, g.out, g.bf16, (uint64_t)g.N, (uint64_t)g.M, (uint64_t)g.N * 2, 32, 32, true))
+      return s;
+    epi.tma_store = 1;
+  }
+  const int64_t tiles = ((g.M + C::BMT - 1) / C::BMT) * ((g.N + BN - 1) / BN);
+  if (tiles >= (1LL << 31)) return fail(FNI8_ERR_UNSUPPORTED, "fp4 GEMM: too many tiles");
+  const int64_t ctas = PAIR ? 2 * tiles : tiles;
+  const int sms = num_sms(dev), cap = PAIR ? (sms & ~1) : sms;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(ctas < cap ? ctas : cap));
+  cfg.blockDim = dim3(fp4::kTileThreads);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled();
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = PAIR ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ta, tb, tsa, tsb, to, epi, (int)g.M, (int)g.N,
+                                           (int)fp4::padded_k(g.K), (int)fp4::k_tiles(FMT, g.K));
+  if (e != cudaSuccess) return cuda_status(e, "launch fp4 gemm");
+  return FNI8_OK;
+}
+
+template <int FMT>
+int pick_tile(const Fp4Gemm& g, cudaStream_t st) {
+  return launch_tile<FMT, 128, false>(g, st);
+}
+
+int run_gemm(const Fp4Gemm& g, cudaStream_t st) {
+  if (g.format == FNI8_MXFP4) return pick_tile<FNI8_MXFP4>(g, st);
+  return pick_tile<FNI8_NVFP4>(g, st);
+}
+
+int check_gemm_fp4(const Fp4Gemm& g, int out_dtype) {
+  if (g.format != FNI8_MXFP4 && g.format != FNI8_NVFP4)
+    return fail(FNI8_ERR_INVALID, "fp4 GEMM: format %d: expected MXFP4 or NVFP4", g.format);
+  if (out_dtype != FNI8_F16 && out_dtype != FNI8_BF16)
+    return fail(FNI8_ERR_INVALID, "out_dtype %d: expected F16 or BF16", out_dtype);
+  if (g.M < 0 || g.N <= 0 || g.K <= 0)
+    return fail(FNI8_ERR_INVALID, "bad GEMM shape M=%lld N=%lld K=%lld", (long long)g.M, (long long)g.N, (long long)g.K);
+  // the scale maps address four rows of 128 bytes per tile with 32-bit coordinates
+  const int64_t lim = 1LL << 31;
+  if (g.M >= lim || g.N >= lim || g.K >= lim ||
+      (fp4::row_tiles(g.M) + 2) * fp4::k_tiles(g.format, g.K) * 4 >= lim ||
+      (fp4::row_tiles(g.N) + 2) * fp4::k_tiles(g.format, g.K) * 4 >= lim)
+    return fail(FNI8_ERR_UNSUPPORTED, "fp4 GEMM: sizes too large");
+  if (g.M == 0) return FNI8_OK;
+  if (!g.a || !g.a_sf || !g.w || !g.w_sf || !g.out) return fail(FNI8_ERR_INVALID, "null GEMM operand");
+  if (g.format == FNI8_NVFP4 && (!g.a_rs || !g.w_rs)) return fail(FNI8_ERR_INVALID, "nvfp4 GEMM: null row scale");
+  if ((reinterpret_cast<uintptr_t>(g.a) | reinterpret_cast<uintptr_t>(g.w) | reinterpret_cast<uintptr_t>(g.a_sf) |
+       reinterpret_cast<uintptr_t>(g.w_sf)) & 15u)
+    return fail(FNI8_ERR_ALIGN, "fp4 GEMM: codes and scales must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(g.out) | reinterpret_cast<uintptr_t>(g.bias)) & 1u)
+    return fail(FNI8_ERR_ALIGN, "fp4 GEMM: out and bias must be 2-byte aligned");
+  return FNI8_OK;
+}
+
+}  // namespace
+}  // namespace fni8h
+
+using namespace fni8h;
+
+extern "C" int fni8_gemm_fp4(const uint8_t* a, const uint8_t* a_sf, const float* a_row_scale, const uint8_t* w,
+                             const uint8_t* w_sf, const float* w_row_scale, const void* bias, void* out, int out_dtype,
+                             int format, int64_t M, int64_t N, int64_t K, void* stream) {
+  const Fp4Gemm g{a, a_sf, a_row_scale, w, w_sf, w_row_scale, bias, out, out_dtype == FNI8_BF16, format, M, N, K};
+  if (int s = check_gemm_fp4(g, out_dtype)) return s;
+  if (M == 0) return FNI8_OK;
+  return run_gemm(g, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int fni8_linear_fp4(const void* x, int dtype, const uint8_t* w, const uint8_t* w_sf, const float* w_row_scale,
+                               const void* bias, void* out, int format, int64_t M, int64_t N, int64_t K,
+                               uint8_t* q_scratch, uint8_t* sf_scratch, float* rs_scratch, void* stream) {
+  if (int s = fp4_check_rows(x, dtype, format, M, K, q_scratch, sf_scratch, rs_scratch)) return s;
+  const Fp4Gemm g{q_scratch, sf_scratch, rs_scratch, w, w_sf, w_row_scale, bias, out, dtype == FNI8_BF16, format, M, N,
+                  K};
+  if (int s = check_gemm_fp4(g, dtype)) return s;
+  if (M == 0) return FNI8_OK;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (int s = fp4_quantize(x, dtype, format, M, K, false, q_scratch, sf_scratch, rs_scratch, st)) return s;
+  return run_gemm(g, st);
+}

@@ -79,6 +79,28 @@ int w4a8_gemm(const int8_t* a, const float* a_scale, const uint8_t* w4, const fl
               void* out, int out_mode, int64_t M, int64_t N, int64_t K, void* ws, size_t ws_bytes, cudaStream_t st);
 int w4a8_status_read_and_clear(int* code);
 
+// 4-bit floating point (fp4.cu: row kernels; gemm_fp4.cu: block-scaled GEMM). Formats and
+// layouts as include/fni8_b200.h documents them.
+struct Fp4Gemm {
+  const uint8_t* a;
+  const uint8_t* a_sf;
+  const float* a_rs;
+  const uint8_t* w;
+  const uint8_t* w_sf;
+  const float* w_rs;
+  const void* bias;
+  void* out;
+  bool bf16;
+  int format;
+  int64_t M, N, K;
+};
+int fp4_check_rows(const void* x, int dtype, int format, int64_t M, int64_t K, const uint8_t* q, const uint8_t* sf,
+                   const float* row_scale);
+// pad: also zero the scales of the rows behind M in the last tile.
+int fp4_quantize(const void* x, int dtype, int format, int64_t M, int64_t K, bool pad, uint8_t* q, uint8_t* sf,
+                 float* row_scale, cudaStream_t st);
+int fp4_status_read_and_clear(int* code);
+
 // Expert-parallel exchange kernels (ep_p2p.cu): capacity-overflow status word.
 int ep_status_read_and_clear(int* code);
 // src [M, N] 16-bit rows (row stride N) to columns [col_off, col_off + N) of each of the

@@ -20,13 +20,14 @@ raises if the library has not been built (there is no fallback path).
 from . import format, mlp, quant  # noqa: F401
 from ._native import Fni8Error
 from .format import FQReader, FQWriter, save_fni8
-from .ops import (act_and_mul, act_and_mul_quant, device_status, gemm_i32, linear, linear_act_q, linear_q,
-                  quantize_rows, rmsnorm, rmsnorm_quant)
+from .ops import (act_and_mul, act_and_mul_quant, dequantize_fp4, device_status, gemm_i32, linear, linear_act_q,
+                  linear_fp4, linear_q, quantize_fp4, quantize_rows, rmsnorm, rmsnorm_quant)
 from .qtensor import QTensor
 
 __all__ = [
     "QTensor", "linear", "rmsnorm", "act_and_mul", "quant",
     "rmsnorm_quant", "act_and_mul_quant", "linear_q", "linear_act_q", "quantize_rows", "gemm_i32", "device_status",
+    "quantize_fp4", "dequantize_fp4", "linear_fp4",
     "Fni8Error", "FQReader", "FQWriter", "save_fni8", "format",
 ]
 __version__ = "0.1.0"

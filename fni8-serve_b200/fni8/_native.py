@@ -16,6 +16,7 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_native", "
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_ALIGN, ERR_CUDA, ERR_WORKSPACE, ERR_DEVICE_TIMEOUT = range(7)
 F16, BF16, F32, I32, I8 = range(5)
 ACT_SILU, ACT_GELU_TANH = 0, 1
+MXFP4, NVFP4 = 0, 1
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 PATH_AUTO, PATH_TILE, PATH_STREAM, PATH_FUSED, PATH_SPLITK = 0, 1, 2, 3, 4
 
@@ -42,6 +43,11 @@ SIGNATURES: dict[str, tuple] = {
     "fni8_act_and_mul_quant_i8_rows": (_i, [_p, _i, _i, _i64, _i64, _p, _p, _p, _p]),
     "fni8_gemm_w4a8": (_i, [_p, _p, _p, _p, _i64, _p, _p, _i, _i64, _i64, _i64, _p, _sz, _p]),
     "fni8_linear_w4a8": (_i, [_p, _i, _p, _p, _i64, _p, _p, _i64, _i64, _i64, _p, _p, _p, _sz, _p]),
+    "fni8_fp4_scale_bytes": (_sz, [_i, _i64, _i64]),
+    "fni8_quantize_rows_fp4": (_i, [_p, _i, _i, _i64, _i64, _p, _p, _p, _p]),
+    "fni8_dequantize_rows_fp4": (_i, [_p, _p, _p, _i, _i64, _i64, _p, _i, _p]),
+    "fni8_gemm_fp4": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i64, _i64, _i64, _p]),
+    "fni8_linear_fp4": (_i, [_p, _i, _p, _p, _p, _p, _p, _i, _i64, _i64, _i64, _p, _p, _p, _p]),
     "fni8_gemm_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "fni8_workspace_init": (_i, [_p, _sz, _p]),
     "fni8_gemm_w8a8": (_i, [_p, _p, _p, _p, _p, _p, _p, _i, _i64, _i64, _i64, _p, _sz, _p]),

@@ -16,7 +16,8 @@ Layout (little-endian): an 8-byte magic, the tensor bytes, each part starting on
 4096-byte boundary, then the JSON header, then a 24-byte footer (header offset, header
 length, magic). Every part is the resident layout the kernels read (per_row_i8: int8
 [N, K] row-major + fp32 scale [N]; per_group_i4: packed uint8 [N, K/2] + fp32 scale
-[N, K/group]; raw: the tensor as is), so a load is a page-aligned read of exactly the
+[N, K/group]; mxfp4 / nvfp4: codes, scale tiles and row scale as fni8.QTensor holds them;
+raw: the tensor as is), so a load is a page-aligned read of exactly the
 requested tensors' bytes and one host-to-device copy: no dequantisation, repacking or
 transposition (the contract of fni8serve/loader.py:1-8). A writer streams tensors to
 disk as they are added, so peak memory is one tensor (fni8serve/convert.py:313-318).
@@ -90,6 +91,10 @@ class FQWriter:
             qt = QTensor(qt, None, scheme="raw")
         entry = {"scheme": qt.scheme, "group_size": qt.group_size, "codebook": qt.codebook,
                  "data": self._part(qt.data), "scale": None if qt.scale is None else self._part(qt.scale)}
+        if qt.row_scale is not None:
+            entry["row_scale"] = self._part(qt.row_scale)
+        if qt.cols is not None:
+            entry["cols"] = int(qt.cols)
         self._entries[name] = entry
 
     def finalize(self, meta: dict | None = None, shards: dict | None = None) -> None:
@@ -98,7 +103,7 @@ class FQWriter:
         meta = dict(meta or {})
         schemes = {e["scheme"] for e in self._entries.values()} - {"raw"}
         quant = ("int8" if schemes == {"per_row_i8"} else "int4" if schemes == {"per_group_i4"} else
-                 "mixed" if schemes else "raw")
+                 next(iter(schemes)) if schemes in ({"mxfp4"}, {"nvfp4"}) else "mixed" if schemes else "raw")
         header = {"version": FORMAT_VERSION, "arch": meta.get("arch", ""), "quant": quant, "__meta__": meta,
                   "shards": shards or {}, "tensors": self._entries}
         cfg = meta.get("config")
@@ -181,7 +186,9 @@ class FQReader:
         e = self._tensors[name]
         data = self._tensor(e["data"], device)
         scale = None if e["scale"] is None else self._tensor(e["scale"], device)
-        return QTensor(data, scale, scheme=e["scheme"], group_size=e["group_size"], codebook=e["codebook"])
+        row = self._tensor(e["row_scale"], device) if e.get("row_scale") is not None else None
+        return QTensor(data, scale, scheme=e["scheme"], group_size=e["group_size"], codebook=e["codebook"],
+                       row_scale=row, cols=e.get("cols"))
 
     def load_many(self, names, device="cpu") -> dict:
         missing = [n for n in names if n not in self._tensors]

@@ -7,7 +7,8 @@ These are the functions fni8-serve's layers import from `fni8`:
     fni8.act_and_mul(x, "silu" | "gelu_tanh")              fni8serve/layers/activation.py:21-41
 
 plus the fused producers the reference does not have (`rmsnorm_quant`,
-`act_and_mul_quant`, `linear_q`) and raw access for tests (`quantize_rows`,
+`act_and_mul_quant`, `linear_q`), 4-bit floating point (`quantize_fp4`, `dequantize_fp4`,
+`linear_fp4`, and `linear` with such weights) and raw access for tests (`quantize_rows`,
 `gemm_i32`). Every op runs on the current CUDA stream, allocates its outputs from the
 PyTorch caching allocator and never synchronises, so the decode step can be captured in
 a CUDA graph as the reference engine does (fni8serve/engine/cuda_graph.py). CPU tensors
@@ -363,14 +364,155 @@ def _linear_w4a8(x: torch.Tensor, qt: QTensor, bias: torch.Tensor | None) -> tor
     return out.reshape(*x.shape[:-1], N)
 
 
+# ------------------------------------------------------------------ 4-bit floating point
+_FP4 = {"mxfp4": (nat.MXFP4, 32), "nvfp4": (nat.NVFP4, 16)}
+
+
+def _fp4_scheme(scheme: str, what: str) -> tuple[int, int]:
+    try:
+        return _FP4[scheme]
+    except KeyError:
+        raise ValueError(f"fni8.{what}: scheme {scheme!r}: expected 'mxfp4' or 'nvfp4'") from None
+
+
+def _fp4_shape(qt: QTensor, what: str) -> tuple[int, int]:
+    """(rows, K) of a quantised matrix whose parts fit together."""
+    _, g = _fp4_scheme(qt.scheme, what)
+    Kp = qt.data.shape[-1] * 2
+    K = Kp if qt.cols is None else int(qt.cols)
+    rows = qt.data.numel() * 2 // Kp if Kp else 0
+    if qt.data.dtype != torch.uint8 or qt.data.dim() < 2 or K <= 0 or (K + 31) // 32 * 32 != Kp:
+        raise ValueError(f"fni8.{what}: {qt.scheme} data {tuple(qt.data.shape)} {qt.data.dtype} does not pack "
+                         f"{K} columns (two codes to a byte, rows padded to 32 values)")
+    if qt.group_size not in (None, g):
+        raise ValueError(f"fni8.{what}: {qt.scheme} has blocks of {g} values (group_size {qt.group_size})")
+    sc = qt.scale
+    if sc is None or sc.dtype != torch.uint8 or sc.numel() != (rows + 127) // 128 * ((K + 4 * g - 1) // (4 * g)) * 512:
+        raise ValueError(f"fni8.{what}: {qt.scheme} scale {None if sc is None else tuple(sc.shape)} is not the tile "
+                         f"order of {rows} x {K} values (fni8.quant.fp4.scale_tiles)")
+    rs = qt.row_scale
+    if qt.scheme == "nvfp4":
+        if rs is None or rs.dtype != torch.float32 or rs.numel() != rows:
+            raise ValueError(f"fni8.{what}: nvfp4 needs row_scale, fp32 [{rows}]")
+    elif rs is not None:
+        raise ValueError(f"fni8.{what}: mxfp4 has no row_scale")
+    if not (qt.data.is_contiguous() and sc.is_contiguous() and (rs is None or rs.is_contiguous())):
+        raise ValueError(f"fni8.{what}: data, scale and row_scale must be contiguous")
+    if sc.device != qt.data.device or (rs is not None and rs.device != qt.data.device):
+        raise RuntimeError(f"fni8.{what}: data, scale and row_scale are on different devices")
+    return rows, K
+
+
+def quantize_fp4(x: torch.Tensor, scheme: str = "mxfp4") -> QTensor:
+    """Rows of x[..., K] to 4-bit floating point: e2m1 codes with one power-of-two scale for
+    every 32 values ("mxfp4", the OCP MX format) or one e4m3 scale for every 16 and a
+    power-of-two scale for each row ("nvfp4"). Returns a QTensor, which `linear_fp4` takes as
+    activations (data keeps the leading dims) and `linear` as a weight (2-D x). Each row
+    depends on itself alone; a block that holds an infinity or a NaN reads back as NaN."""
+    _need_cuda(x, "quantize_fp4")
+    dt = _act_dtype(x, "quantize_fp4")
+    fmt, g = _fp4_scheme(scheme, "quantize_fp4")
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError("fni8.quantize_fp4: empty rows")
+    K, lead, dev = x.shape[-1], x.shape[:-1], x.device
+    x2 = x.reshape(-1, K).contiguous()
+    M = x2.shape[0]
+    q = torch.empty((M, (K + 31) // 32 * 16), dtype=torch.uint8, device=dev)
+    sf = torch.empty(((M + 127) // 128, (K + 4 * g - 1) // (4 * g), 512), dtype=torch.uint8, device=dev)
+    rs = torch.empty((M,), dtype=torch.float32, device=dev) if scheme == "nvfp4" else None
+    with torch.cuda.device(dev):
+        nat.call("fni8_quantize_rows_fp4", _vp(x2), dt, fmt, M, K, _vp(q), _vp(sf), _vp(rs), _stream(dev))
+    return QTensor(q.reshape(*lead, q.shape[1]) if x.dim() != 2 else q, sf, scheme=scheme, group_size=g,
+                   row_scale=rs if rs is None or x.dim() == 2 else rs.reshape(lead), cols=K)
+
+
+def dequantize_fp4(qt: QTensor, dtype: torch.dtype = torch.float16) -> torch.Tensor:
+    """The values [..., K] of an mxfp4 or nvfp4 QTensor, rounded once to dtype (float16,
+    bfloat16 or float32)."""
+    _need_cuda(qt.data, "dequantize_fp4")
+    M, K = _fp4_shape(qt, "dequantize_fp4")
+    odt = {torch.float16: nat.F16, torch.bfloat16: nat.BF16, torch.float32: nat.F32}.get(dtype)
+    if odt is None:
+        raise TypeError(f"fni8.dequantize_fp4: dtype must be float16, bfloat16 or float32, got {dtype}")
+    dev = qt.data.device
+    out = torch.empty((*qt.data.shape[:-1], K), dtype=dtype, device=dev)
+    with torch.cuda.device(dev):
+        nat.call("fni8_dequantize_rows_fp4", _vp(qt.data), _vp(qt.scale), _vp(qt.row_scale), _FP4[qt.scheme][0], M, K,
+                 _vp(out), odt, _stream(dev))
+    return out
+
+
+def _fp4_weight(qt: QTensor, K: int, dev: torch.device, what: str) -> int:
+    N, Kw = _fp4_shape(qt, what)
+    if qt.data.dim() != 2:
+        raise ValueError(f"fni8.{what}: a weight is 2-D, got {tuple(qt.data.shape)}")
+    if Kw != K:
+        raise ValueError(f"fni8.{what}: in_features {Kw} != activation K {K}")
+    if qt.data.device != dev:
+        raise RuntimeError(f"fni8.{what}: weight and activation are on different devices")
+    return N
+
+
+def _fp4_bias(bias: torch.Tensor | None, N: int, dtype: torch.dtype, dev: torch.device, what: str):
+    if bias is None:
+        return None
+    if bias.numel() != N or bias.device != dev:
+        raise ValueError(f"fni8.{what}: bias must hold {N} values on {dev}")
+    return bias.to(dtype).contiguous()
+
+
+def linear_fp4(xq: QTensor, qt: QTensor, bias: torch.Tensor | None = None,
+               out_dtype: torch.dtype = torch.float16) -> torch.Tensor:
+    """y[..., N] = xq . qt^T (+ bias) for activations and a weight quantised by quantize_fp4
+    to the same scheme: summed in fp32 by the block-scaled tensor core, rounded once."""
+    _need_cuda(xq.data, "linear_fp4")
+    if xq.scheme != qt.scheme:
+        raise ValueError(f"fni8.linear_fp4: activations {xq.scheme}, weight {qt.scheme}")
+    if out_dtype not in _DT:
+        raise TypeError(f"fni8.linear_fp4: out_dtype must be float16 or bfloat16, got {out_dtype}")
+    M, K = _fp4_shape(xq, "linear_fp4")
+    dev = xq.data.device
+    N = _fp4_weight(qt, K, dev, "linear_fp4")
+    b = _fp4_bias(bias, N, out_dtype, dev, "linear_fp4")
+    out = torch.empty((*xq.data.shape[:-1], N), dtype=out_dtype, device=dev)
+    with torch.cuda.device(dev):
+        nat.call("fni8_gemm_fp4", _vp(xq.data), _vp(xq.scale), _vp(xq.row_scale), _vp(qt.data), _vp(qt.scale),
+                 _vp(qt.row_scale), _vp(b), _vp(out), _DT[out_dtype], _FP4[qt.scheme][0], M, N, K, _stream(dev))
+    return out
+
+
+def _linear_fp4(x: torch.Tensor, qt: QTensor, bias: torch.Tensor | None) -> torch.Tensor:
+    """mxfp4 / nvfp4 weights: x's rows quantised to the same scheme, then the block-scaled GEMM."""
+    dt = _act_dtype(x, "linear")
+    fmt, g = _FP4[qt.scheme]
+    K, dev = x.shape[-1], x.device
+    N = _fp4_weight(qt, K, dev, "linear")
+    x2 = x.reshape(-1, K).contiguous()
+    M = x2.shape[0]
+    b = _fp4_bias(bias, N, x.dtype, dev, "linear")
+    out = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev)
+    # one scratch: scale tiles, codes, row scales (each part a multiple of 16 bytes)
+    sf_bytes = (M + 127) // 128 * ((K + 4 * g - 1) // (4 * g)) * 512
+    q_bytes = M * ((K + 31) // 32 * 16)
+    scratch = torch.empty(sf_bytes + q_bytes + 4 * M, dtype=torch.uint8, device=dev)
+    sf = scratch.data_ptr()
+    with torch.cuda.device(dev):
+        nat.call("fni8_linear_fp4", _vp(x2), dt, _vp(qt.data), _vp(qt.scale), _vp(qt.row_scale), _vp(b), _vp(out), fmt,
+                 M, N, K, sf + sf_bytes, sf, sf + sf_bytes + q_bytes, _stream(dev))
+    return out
+
+
 def linear(x: torch.Tensor, qt: QTensor, bias: torch.Tensor | None = None, path: int = nat.PATH_AUTO) -> torch.Tensor:
     """fni8.linear: per-token int8 quantisation of x, int8 GEMM, dequant epilogue (+bias).
 
     `path` (not in the reference signature) forces a kernel; the default picks by shape.
-    per_group_i4 / int4 weights run the W4A8 GEMM."""
+    per_group_i4 / int4 weights run the W4A8 GEMM; mxfp4 / nvfp4 weights quantise x to their
+    own format instead and run the block-scaled GEMM."""
     _need_cuda(x, "linear")
     if qt.scheme == "per_group_i4":
         return _linear_w4a8(x, qt, bias)
+    if qt.scheme in _FP4:
+        return _linear_fp4(x, qt, bias)
     dt = _act_dtype(x, "linear")
     K = x.shape[-1]
     _check_weight(qt, x.device, K, "linear")

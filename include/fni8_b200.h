@@ -63,6 +63,11 @@ enum fni8_status {
 enum fni8_dtype { FNI8_F16 = 0, FNI8_BF16 = 1, FNI8_F32 = 2, FNI8_I32 = 3, FNI8_I8 = 4 };
 enum fni8_act { FNI8_ACT_SILU = 0, FNI8_ACT_GELU_TANH = 1 };
 enum fni8_scoring { FNI8_SCORE_SOFTMAX = 0, FNI8_SCORE_SIGMOID = 1 };
+/* 4-bit floating point formats (e2m1 codes with block scales). */
+enum fni8_fp4 {
+  FNI8_MXFP4 = 0, /* OCP MX: one e8m0 scale (a power of two) for every 32 values */
+  FNI8_NVFP4 = 1  /* one e4m3 scale for every 16 values, one fp32 scale for each row */
+};
 /* GEMM kernel selection (fni8_gemm_w8a8_ex). AUTO picks by shape. */
 enum fni8_gemm_path {
   FNI8_PATH_AUTO = 0,   /* by shape, from B200 measurements */
@@ -224,6 +229,54 @@ FNI8_API int fni8_gemm_w4a8(const int8_t* a, const float* a_scale, const uint8_t
 FNI8_API int fni8_linear_w4a8(const void* x, int dtype, const uint8_t* w4, const float* w_scale, int64_t group_size,
                               const void* bias, void* out, int64_t M, int64_t N, int64_t K, int8_t* q_scratch,
                               float* s_scratch, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------ 4-bit floating point
+ * New capability (the reference's 4-bit weights are integer or NF4 groups with 8-bit
+ * activations, fni8serve/layers/linear.py:33-45): weights and activations in e2m1
+ * (magnitudes 0, 0.5, 1, 1.5, 2, 3, 4, 6) with block scales, multiplied by the block-scaled
+ * tensor core.
+ *
+ * Layout of a quantised matrix [M, K]:
+ *  - q: two codes to a byte, the even element in the low half; rows of Kp / 2 bytes, Kp = K
+ *    rounded up to 32, zero codes behind K.
+ *  - sf: one byte for every block of g values (g = 32 for FNI8_MXFP4, 16 for FNI8_NVFP4), in
+ *    tiles of 128 rows x 4 scales, 512 bytes each; tile (r / 128, s / 4) of row r and scale s
+ *    is number (r / 128) * ceil(ceil(K / g) / 4) + s / 4, and within it the byte is
+ *    (r % 32) * 16 + (r % 128 / 32) * 4 + s % 4. Scales behind K are zero; those of rows
+ *    behind M are zero from fni8_quantize_rows_fp4, and are never used.
+ *  - row_scale: fp32 [M] for FNI8_NVFP4, NULL for FNI8_MXFP4.
+ * A value is e2m1(code) * sf (* row_scale). An sf of NaN (0xFF for e8m0, 0x7F for e4m3)
+ * makes its block, and every output that it enters, NaN. */
+/* Bytes of the scale tiles of an [M, K] matrix (0 for an unknown format or size). */
+FNI8_API size_t fni8_fp4_scale_bytes(int format, int64_t M, int64_t K);
+
+/* Rows of x[M, K] (F16 or BF16) to 4-bit floating point.
+ *  FNI8_MXFP4 (OCP Microscaling Formats 1.0, section 6.3): e = floor(log2(max |block|)) - 2
+ *   within [-127, 127], code = e2m1(x / 2^e), rounded to nearest even, at most 6.
+ *  FNI8_NVFP4: row_scale = the least power of two (>= 2^-126) with
+ *   max |row| / row_scale <= 2688 = 6 * 448, sf = e4m3(max |block| / (6 row_scale)) rounded
+ *   to nearest even, code = e2m1(x / (row_scale sf)) likewise (0 where sf is 0).
+ * Both are exact: the codes are those of the real quotients. A block that holds an infinity
+ * or a NaN gets the scale NaN, and does not enter its row's maximum. Any K. */
+FNI8_API int fni8_quantize_rows_fp4(const void* x, int dtype, int format, int64_t M, int64_t K, uint8_t* q,
+                                    uint8_t* sf, float* row_scale, void* stream);
+/* The values of a quantised matrix, rounded once to out_dtype (F16, BF16 or F32): out[M, K]. */
+FNI8_API int fni8_dequantize_rows_fp4(const uint8_t* q, const uint8_t* sf, const float* row_scale, int format,
+                                      int64_t M, int64_t K, void* out, int out_dtype, void* stream);
+
+/* out[M, N] = a . w^T for quantised a[M, K] and w[N, K] of one format: the block-scaled sum
+ * in fp32, then (sum * a_row_scale[m]) * w_row_scale[n] (+ bias[n]), rounded once to
+ * out_dtype (F16 or BF16; bias in out_dtype or NULL). q rows 16-byte aligned. No workspace:
+ * concurrent calls are independent. */
+FNI8_API int fni8_gemm_fp4(const uint8_t* a, const uint8_t* a_sf, const float* a_row_scale, const uint8_t* w,
+                           const uint8_t* w_sf, const float* w_row_scale, const void* bias, void* out, int out_dtype,
+                           int format, int64_t M, int64_t N, int64_t K, void* stream);
+/* fni8.linear(x, qt, bias=) for FNI8_MXFP4 / FNI8_NVFP4 weights: x[M, K] quantised to the
+ * weight's format into q_scratch [M, Kp / 2], sf_scratch (fni8_fp4_scale_bytes) and, for
+ * FNI8_NVFP4, rs_scratch [M], then fni8_gemm_fp4 into out[M, N] (dtype of x). */
+FNI8_API int fni8_linear_fp4(const void* x, int dtype, const uint8_t* w, const uint8_t* w_sf, const float* w_row_scale,
+                             const void* bias, void* out, int format, int64_t M, int64_t N, int64_t K,
+                             uint8_t* q_scratch, uint8_t* sf_scratch, float* rs_scratch, void* stream);
 
 /* ------------------------------------------------------------------ MoE */
 /* Router scores -> top-k (SparseMoE.forward routing, fni8serve/models/moe.py:65-95):
