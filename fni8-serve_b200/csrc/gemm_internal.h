@@ -101,6 +101,33 @@ int fp4_quantize(const void* x, int dtype, int format, int64_t M, int64_t K, boo
                  float* row_scale, cudaStream_t st);
 int fp4_status_read_and_clear(int* code);
 
+// The routed-expert layer for a few tokens in two kernels (moe_few.cu). logits null: the
+// routing topi / topw is given. h: scratch [T k, I] of the activations' type, 16-byte aligned,
+// as x is.
+struct FewMoe {
+  const void* x;
+  int dtype;
+  int64_t T, H, E, I, k;
+  const float* logits;
+  const int32_t* topi;
+  const float* topw;
+  int scoring;
+  const float* sel_bias;
+  int64_t n_groups, topk_group;
+  int norm_topk;
+  float scaling;
+  const int8_t* w_gu;
+  const float* s_gu;
+  const int8_t* w_dn;
+  const float* s_dn;
+  int act;
+  void* h;
+  void* out;
+};
+bool few_supported(int64_t T, int64_t H, int64_t k, int64_t E, int64_t I);
+int few_moe(const FewMoe& m, cudaStream_t st);
+int few_status_read_and_clear(int* code);
+
 // Expert-parallel exchange kernels (ep_p2p.cu): capacity-overflow status word.
 int ep_status_read_and_clear(int* code);
 // src [M, N] 16-bit rows (row stride N) to columns [col_off, col_off + N) of each of the

@@ -15,6 +15,7 @@
 // Nothing here waits on another CTA, so there is no watchdog word in this file.
 #include "fni8_common.cuh"
 #include "gemm_internal.h"
+#include "moe_route.cuh"
 
 namespace fni8b {
 namespace moe {
@@ -22,29 +23,6 @@ namespace moe {
 constexpr int kMaxE = 1024;
 constexpr int kMaxK = 32;
 constexpr int kChunk = 1024;  // slots per plan CTA
-
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
-// warp-wide arg-max: larger value wins, ties go to the lower index
-__device__ __forceinline__ void warp_argmax(float& v, int& i) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float ov = __shfl_xor_sync(0xffffffffu, v, o);
-    const int oi = __shfl_xor_sync(0xffffffffu, i, o);
-    if (ov > v || (ov == v && oi < i)) {
-      v = ov;
-      i = oi;
-    }
-  }
-}
 
 // VPL = experts per lane (E <= 32 * VPL).
 template <int VPL>
@@ -57,108 +35,13 @@ __global__ void route_kernel(const float* __restrict__ logits, int T, int E, int
   const int t = blockIdx.x * warps + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (t >= T) return;
-  const float* lr = logits + static_cast<int64_t>(t) * E;
-  const float NEG = -INFINITY;
-  float sc[VPL], sel[VPL];
-#pragma unroll
-  for (int i = 0; i < VPL; ++i) {
-    const int e = lane + 32 * i;
-    sc[i] = e < E ? lr[e] : NEG;
-  }
-  if (scoring == FNI8_SCORE_SOFTMAX) {
-    float mx = NEG;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) mx = fmaxf(mx, sc[i]);
-    mx = warp_max(mx);
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const int e = lane + 32 * i;
-      sc[i] = e < E ? expf(__fadd_rn(sc[i], -mx)) : 0.0f;
-      sum = __fadd_rn(sum, sc[i]);
-    }
-    sum = warp_sum(sum);
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      sc[i] = __fdiv_rn(sc[i], sum);
-      sel[i] = (lane + 32 * i) < E ? sc[i] : NEG;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const int e = lane + 32 * i;
-      sc[i] = e < E ? __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-sc[i]))) : 0.0f;
-      sel[i] = e < E ? (sel_bias ? __fadd_rn(sc[i], sel_bias[e]) : sc[i]) : NEG;
-    }
-  }
-  if (n_groups > 0 && topk_group > 0) {
-    // keep only the topk_group groups with the largest max score
-    const int epg = E / n_groups;
-    unsigned keep = 0;  // bitmask over groups (n_groups <= 32)
-    for (int r = 0; r < topk_group; ++r) {
-      float best = NEG;
-      int bg = 0x7fffffff;
-      for (int g = 0; g < n_groups; ++g) {
-        if (keep & (1u << g)) continue;
-        float gm = NEG;
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) {
-          const int e = lane + 32 * i;
-          if (e < E && e / epg == g) gm = fmaxf(gm, sel[i]);
-        }
-        gm = warp_max(gm);
-        if (gm > best) {
-          best = gm;
-          bg = g;
-        }
-      }
-      if (bg != 0x7fffffff) keep |= 1u << bg;
-    }
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const int e = lane + 32 * i;
-      if (e < E && !(keep & (1u << (e / epg)))) sel[i] = NEG;
-    }
-  }
-  float my_w = 0.0f;
   int my_i = 0;
-  float wsum = 0.0f;
-  for (int j = 0; j < k; ++j) {
-    float v = NEG;
-    int idx = 0x7fffffff;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const int e = lane + 32 * i;
-      if (e < E && (sel[i] > v || (sel[i] == v && e < idx))) {
-        v = sel[i];
-        idx = e;
-      }
-    }
-    warp_argmax(v, idx);
-    float w = 0.0f;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      if (lane + 32 * i == idx) {
-        w = sc[i];
-        sel[i] = NEG;  // taken
-        // a -inf entry can only be re-picked if everything left is -inf; mark it below E
-      }
-    }
-    w = __shfl_sync(0xffffffffu, w, idx & 31);
-    if (lane == j) {  // slot j stays in lane j (k <= 32)
-      my_w = w;
-      my_i = idx;
-    }
-    wsum = __fadd_rn(wsum, w);  // in slot order, as the reference's sum over k
-  }
+  float my_w = 0.0f;
+  route_token<VPL>(logits + static_cast<int64_t>(t) * E, E, k, scoring, sel_bias, n_groups, topk_group, norm_topk,
+                   scaling, wdtype, lane, my_i, my_w);
   if (lane < k) {
-    const float denom = fmaxf(wsum, 1e-9f);
-    float w = norm_topk ? __fdiv_rn(my_w, denom) : my_w;
-    w = __fmul_rn(w, scaling);
-    if (wdtype == FNI8_F16) w = __half2float(__float2half_rn(w));
-    else if (wdtype == FNI8_BF16) w = __bfloat162float(__float2bfloat16_rn(w));
     topi[static_cast<int64_t>(t) * k + lane] = my_i;
-    topw[static_cast<int64_t>(t) * k + lane] = w;
+    topw[static_cast<int64_t>(t) * k + lane] = my_w;
   }
 }
 
@@ -358,9 +241,8 @@ using namespace fni8h;
 
 static size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
-extern "C" int fni8_moe_route(const float* logits, int64_t T, int64_t E, int64_t top_k, int scoring,
-                              const float* sel_bias, int64_t n_groups, int64_t topk_group, int norm_topk,
-                              float scaling, int weight_dtype, int32_t* topi, float* topw, void* stream) {
+static int check_route(int64_t T, int64_t E, int64_t top_k, int scoring, int64_t n_groups, int64_t topk_group,
+                       int weight_dtype) {
   if (T < 0 || E <= 0 || E > moe::kMaxE) return fail(FNI8_ERR_INVALID, "route: need 0 < E <= %d", moe::kMaxE);
   if (top_k <= 0 || top_k > moe::kMaxK || top_k > E) return fail(FNI8_ERR_INVALID, "route: bad top_k %lld", (long long)top_k);
   if (scoring != FNI8_SCORE_SOFTMAX && scoring != FNI8_SCORE_SIGMOID) return fail(FNI8_ERR_INVALID, "route: scoring");
@@ -368,6 +250,13 @@ extern "C" int fni8_moe_route(const float* logits, int64_t T, int64_t E, int64_t
     return fail(FNI8_ERR_INVALID, "route: bad expert grouping");
   if (weight_dtype != FNI8_F16 && weight_dtype != FNI8_BF16 && weight_dtype != FNI8_F32)
     return fail(FNI8_ERR_INVALID, "route: weight_dtype");
+  return FNI8_OK;
+}
+
+extern "C" int fni8_moe_route(const float* logits, int64_t T, int64_t E, int64_t top_k, int scoring,
+                              const float* sel_bias, int64_t n_groups, int64_t topk_group, int norm_topk,
+                              float scaling, int weight_dtype, int32_t* topi, float* topw, void* stream) {
+  if (int s = check_route(T, E, top_k, scoring, n_groups, topk_group, weight_dtype)) return s;
   if (T == 0) return FNI8_OK;
   if (logits == nullptr || topi == nullptr || topw == nullptr) return fail(FNI8_ERR_INVALID, "route: null pointer");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -577,6 +466,13 @@ extern "C" size_t fni8_moe_experts_workspace_bytes(int64_t T, int64_t H, int64_t
   return moe_layout(T, H, top_k, E, I).total;
 }
 
+// Whether a call takes the two-kernel form. (Anything else, wrong arguments included, is for
+// the composed path below, whose results are the same.)
+static bool few_tokens(const void* x, int act, int64_t T, int64_t H, int64_t k, int64_t E, int64_t I) {
+  return (act == FNI8_ACT_SILU || act == FNI8_ACT_GELU_TANH) && (reinterpret_cast<uintptr_t>(x) & 15u) == 0 &&
+         few_supported(T, H, k, E, I);
+}
+
 extern "C" int fni8_moe_experts_w8a8(const void* x, int dtype, int64_t T, int64_t H, const int32_t* topi,
                                      const float* topw, int64_t top_k, const int8_t* w_gu, const float* s_gu,
                                      const int8_t* w_dn, const float* s_dn, int64_t E, int64_t I, int act, void* out,
@@ -605,6 +501,9 @@ extern "C" int fni8_moe_experts_w8a8(const void* x, int dtype, int64_t T, int64_
   void* y = b + L.y;
   const int64_t R = T * top_k;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (few_tokens(x, act, T, H, top_k, E, I))
+    return few_moe({x, dtype, T, H, E, I, top_k, nullptr, topi, topw, 0, nullptr, 0, 0, 0, 1.0f, w_gu, s_gu, w_dn, s_dn,
+                    act, h, out}, st);
   // plan first (with the segment tables), then each token is quantised once and its int8
   // row written straight to the grouped rows of its slots (no [T, H] int8 copy, no gather)
   if (int s = moe_plan(topi, R, E, counts, offsets, ros, sor, b + L.plan, L.counts - L.plan, tables, stream))
@@ -628,4 +527,41 @@ extern "C" int fni8_moe_experts_w8a8(const void* x, int dtype, int64_t T, int64_
   if (int s = fni8_grouped_gemm_w8a8(hq, hs, R, w_dn, s_dn, E, H, I, seg_e, offsets, counts, E, y, dtype, stream))
     return s;
   return fni8_moe_combine(y, dtype, ros, topw, T, top_k, H, out, stream);
+}
+
+extern "C" size_t fni8_moe_layer_workspace_bytes(int64_t T, int64_t H, int64_t top_k, int64_t E, int64_t I) {
+  const size_t b = fni8_moe_experts_workspace_bytes(T, H, top_k, E, I);
+  return b == 0 ? 0 : b + 2 * align256(static_cast<size_t>(T) * top_k * 4);
+}
+
+extern "C" int fni8_moe_layer_w8a8(const void* x, int dtype, int64_t T, int64_t H, const float* logits, int64_t top_k,
+                                   int scoring, const float* sel_bias, int64_t n_groups, int64_t topk_group,
+                                   int norm_topk, float scaling, const int8_t* w_gu, const float* s_gu,
+                                   const int8_t* w_dn, const float* s_dn, int64_t E, int64_t I, int act, void* out,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+  if (dtype != FNI8_F16 && dtype != FNI8_BF16) return fail(FNI8_ERR_INVALID, "moe: dtype");
+  if (T < 0 || H <= 0 || top_k <= 0 || E <= 0 || I <= 0) return fail(FNI8_ERR_INVALID, "moe: bad sizes");
+  if (act != FNI8_ACT_SILU && act != FNI8_ACT_GELU_TANH) return fail(FNI8_ERR_INVALID, "unknown activation %d", act);
+  if (int s = check_route(T, E, top_k, scoring, n_groups, topk_group, dtype)) return s;
+  if (E > kTileMaxSeg) return fail(FNI8_ERR_UNSUPPORTED, "moe: at most %d experts", kTileMaxSeg);
+  if (H % 16 != 0 || I % 16 != 0) return fail(FNI8_ERR_UNSUPPORTED, "moe: H and I must be multiples of 16");
+  if (T == 0) return FNI8_OK;
+  if (!x || !logits || !w_gu || !s_gu || !w_dn || !s_dn || !out) return fail(FNI8_ERR_INVALID, "moe: null pointer");
+  const size_t need = fni8_moe_layer_workspace_bytes(T, H, top_k, E, I);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(FNI8_ERR_WORKSPACE, "moe needs %zu workspace bytes (got %zu)", need, workspace_bytes);
+  if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail(FNI8_ERR_ALIGN, "moe: workspace must be 256-byte aligned");
+  if (few_tokens(x, act, T, H, top_k, E, I))
+    return few_moe({x, dtype, T, H, E, I, top_k, logits, nullptr, nullptr, scoring, sel_bias, n_groups, topk_group,
+                    norm_topk, scaling, w_gu, s_gu, w_dn, s_dn, act,
+                    static_cast<uint8_t*>(workspace) + moe_layout(T, H, top_k, E, I).h, out},
+                   static_cast<cudaStream_t>(stream));
+  const size_t part = align256(static_cast<size_t>(T) * top_k * 4), base = need - 2 * part;
+  int32_t* topi = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + base);
+  float* topw = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + base + part);
+  if (int s = fni8_moe_route(logits, T, E, top_k, scoring, sel_bias, n_groups, topk_group, norm_topk, scaling, dtype,
+                             topi, topw, stream))
+    return s;
+  return fni8_moe_experts_w8a8(x, dtype, T, H, topi, topw, top_k, w_gu, s_gu, w_dn, s_dn, E, I, act, out, workspace,
+                               base, stream);
 }

@@ -1,0 +1,144 @@
+// Routing of one token by one warp (fni8serve/models/moe.py:65-95): shared by the routing
+// kernel (moe.cu) and the few-token layer (moe_few.cu), so both choose alike.
+#pragma once
+#include "fni8_common.cuh"
+
+namespace fni8b {
+namespace moe {
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+// warp-wide arg-max: larger value wins, ties go to the lower index
+__device__ __forceinline__ void warp_argmax(float& v, int& i) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float ov = __shfl_xor_sync(0xffffffffu, v, o);
+    const int oi = __shfl_xor_sync(0xffffffffu, i, o);
+    if (ov > v || (ov == v && oi < i)) {
+      v = ov;
+      i = oi;
+    }
+  }
+}
+
+// Scores of logits row `lr` [E] and the top k of them: lane j < k returns slot j's expert in
+// `out_i` and its weight in `out_w`. VPL = experts per lane (E <= 32 * VPL).
+template <int VPL>
+__device__ __forceinline__ void route_token(const float* __restrict__ lr, int E, int k, int scoring,
+                                            const float* __restrict__ sel_bias, int n_groups, int topk_group,
+                                            int norm_topk, float scaling, int wdtype, int lane, int& out_i,
+                                            float& out_w) {
+  const float NEG = -INFINITY;
+  float sc[VPL], sel[VPL];
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    const int e = lane + 32 * i;
+    sc[i] = e < E ? lr[e] : NEG;
+  }
+  if (scoring == FNI8_SCORE_SOFTMAX) {
+    float mx = NEG;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) mx = fmaxf(mx, sc[i]);
+    mx = warp_max(mx);
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const int e = lane + 32 * i;
+      sc[i] = e < E ? expf(__fadd_rn(sc[i], -mx)) : 0.0f;
+      sum = __fadd_rn(sum, sc[i]);
+    }
+    sum = warp_sum(sum);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      sc[i] = __fdiv_rn(sc[i], sum);
+      sel[i] = (lane + 32 * i) < E ? sc[i] : NEG;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const int e = lane + 32 * i;
+      sc[i] = e < E ? __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-sc[i]))) : 0.0f;
+      sel[i] = e < E ? (sel_bias ? __fadd_rn(sc[i], sel_bias[e]) : sc[i]) : NEG;
+    }
+  }
+  if (n_groups > 0 && topk_group > 0) {
+    // keep only the topk_group groups with the largest max score
+    const int epg = E / n_groups;
+    unsigned keep = 0;  // bitmask over groups (n_groups <= 32)
+    for (int r = 0; r < topk_group; ++r) {
+      float best = NEG;
+      int bg = 0x7fffffff;
+      for (int g = 0; g < n_groups; ++g) {
+        if (keep & (1u << g)) continue;
+        float gm = NEG;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+          const int e = lane + 32 * i;
+          if (e < E && e / epg == g) gm = fmaxf(gm, sel[i]);
+        }
+        gm = warp_max(gm);
+        if (gm > best) {
+          best = gm;
+          bg = g;
+        }
+      }
+      if (bg != 0x7fffffff) keep |= 1u << bg;
+    }
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const int e = lane + 32 * i;
+      if (e < E && !(keep & (1u << (e / epg)))) sel[i] = NEG;
+    }
+  }
+  float my_w = 0.0f;
+  int my_i = 0;
+  float wsum = 0.0f;
+  for (int j = 0; j < k; ++j) {
+    float v = NEG;
+    int idx = 0x7fffffff;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const int e = lane + 32 * i;
+      if (e < E && (sel[i] > v || (sel[i] == v && e < idx))) {
+        v = sel[i];
+        idx = e;
+      }
+    }
+    warp_argmax(v, idx);
+    float w = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      if (lane + 32 * i == idx) {
+        w = sc[i];
+        sel[i] = NEG;  // taken
+        // a -inf entry can only be re-picked if everything left is -inf; mark it below E
+      }
+    }
+    w = __shfl_sync(0xffffffffu, w, idx & 31);
+    if (lane == j) {  // slot j stays in lane j (k <= 32)
+      my_w = w;
+      my_i = idx;
+    }
+    wsum = __fadd_rn(wsum, w);  // in slot order, as the reference's sum over k
+  }
+  if (lane < k) {
+    const float denom = fmaxf(wsum, 1e-9f);
+    float w = norm_topk ? __fdiv_rn(my_w, denom) : my_w;
+    w = __fmul_rn(w, scaling);
+    if (wdtype == FNI8_F16) w = __half2float(__float2half_rn(w));
+    else if (wdtype == FNI8_BF16) w = __bfloat162float(__float2bfloat16_rn(w));
+    out_i = my_i;
+    out_w = w;
+  }
+}
+
+}  // namespace moe
+}  // namespace fni8b

@@ -88,16 +88,6 @@ __device__ __forceinline__ float block_reduce_sum(float v, float* red) {
   return r;
 }
 
-// scale = absmax / 127 is what the GEMM epilogue multiplies with; the codes are
-// round_half_even(x * (127 / absmax)) — one reciprocal per row instead of a division per
-// element (measured: the per-element IEEE division halved the quantiser's throughput).
-__device__ __forceinline__ float quant_scale(float amax) { return __fdiv_rn(amax, 127.0f); }
-__device__ __forceinline__ float quant_inv(float amax) { return amax > 0.0f ? __fdiv_rn(127.0f, amax) : 0.0f; }
-__device__ __forceinline__ int8_t quant_one(float v, float inv) {
-  float q = rintf(__fmul_rn(v, inv));
-  q = fminf(fmaxf(q, -127.0f), 127.0f);
-  return static_cast<int8_t>(static_cast<int>(q));
-}
 __device__ __forceinline__ uint2 quant8(const float (&f)[8], float inv) {
   uint32_t lo = 0, hi = 0;
 #pragma unroll

@@ -72,6 +72,9 @@ SIGNATURES: dict[str, tuple] = {
     "fni8_moe_experts_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
     "fni8_moe_experts_w8a8": (_i, [_p, _i, _i64, _i64, _p, _p, _i64, _p, _p, _p, _p, _i64, _i64, _i, _p, _p, _sz,
                                    _p]),
+    "fni8_moe_layer_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
+    "fni8_moe_layer_w8a8": (_i, [_p, _i, _i64, _i64, _p, _i64, _i, _p, _i64, _i64, _i, _f, _p, _p, _p, _p, _i64, _i64,
+                                 _i, _p, _p, _sz, _p]),
     "fni8_ipc_alloc": (_i, [_sz, ctypes.POINTER(_p), _p]),
     "fni8_ipc_free": (_i, [_p]),
     "fni8_ipc_open": (_i, [_p, ctypes.POINTER(_p)]),

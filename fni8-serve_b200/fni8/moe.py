@@ -17,6 +17,9 @@ pipeline without host synchronisation (capturable in a CUDA graph):
 `SparseMoE` below takes the reference module's constructor arguments unchanged
 (moe.py:25-60), so `fni8serve.models.moe.SparseMoE = fni8.moe.SparseMoE` (or the
 one-line import swap in that file) moves every MoE family onto the grouped kernels.
+
+`layer` is that pipeline in one call. Up to 16 tokens (a decode step) it runs in two kernels
+that stream each active expert's weights once, with the same results bit for bit.
 """
 from __future__ import annotations
 
@@ -182,6 +185,45 @@ def experts(x: torch.Tensor, topi: torch.Tensor, topw: torch.Tensor, stack: Expe
     return out
 
 
+def layer(x: torch.Tensor, logits: torch.Tensor, stack: ExpertStack, top_k: int, *, scoring: str = "softmax",
+          sel_bias: torch.Tensor | None = None, num_expert_groups: int | None = None, topk_group: int | None = None,
+          norm_topk_prob: bool = True, scaling: float = 1.0, act: str = "silu") -> torch.Tensor:
+    """The routed layer from the router's logits on: experts(x, *route(logits, ...), stack), bit
+    for bit, in one native call; up to 16 tokens in two kernels (moe_few.cu). x [T, H],
+    logits [T, E]; the other arguments as in `route` (weights are rounded to x.dtype)."""
+    _need_cuda(x, "moe.layer")
+    if act not in _ACT:
+        raise ValueError(f"unknown activation {act!r}")
+    if scoring not in ("softmax", "sigmoid"):
+        raise ValueError(f"unknown scoring_func {scoring!r}")
+    if x.dtype not in _DT:
+        raise TypeError(f"fni8.moe.layer: activations must be float16 or bfloat16, got {x.dtype}")
+    E, I = stack.num_experts, stack.intermediate
+    if x.dim() != 2 or x.shape[1] != stack.hidden or logits.shape != (x.shape[0], E):
+        raise ValueError(f"fni8.moe.layer: x {tuple(x.shape)} and logits {tuple(logits.shape)} do not fit "
+                         f"{E} experts of hidden size {stack.hidden}")
+    dev = x.device
+    if logits.device != dev or stack.w_gu.device != dev:
+        raise RuntimeError("fni8.moe.layer: x, logits and experts are on different devices")
+    x2, lg = x.contiguous(), logits.float().contiguous()
+    T, H = x2.shape
+    bias = None
+    if sel_bias is not None and scoring == "sigmoid":
+        if sel_bias.numel() != E or sel_bias.device != dev:
+            raise ValueError(f"fni8.moe.layer: sel_bias must hold {E} values on {dev}")
+        bias = sel_bias.float().contiguous()
+    ng = int(num_expert_groups) if (num_expert_groups is not None and topk_group is not None) else 0
+    wsb = nat.lib().fni8_moe_layer_workspace_bytes(T, H, top_k, E, I)
+    ws = torch.empty(max(wsb, 1), dtype=torch.uint8, device=dev)
+    out = torch.empty_like(x2)
+    with torch.cuda.device(dev):
+        nat.call("fni8_moe_layer_w8a8", _vp(x2), _DT[x.dtype], T, H, _vp(lg), top_k,
+                 nat.SCORE_SOFTMAX if scoring == "softmax" else nat.SCORE_SIGMOID, _vp(bias), ng,
+                 int(topk_group) if ng else 0, int(norm_topk_prob), scaling, _vp(stack.w_gu), _vp(stack.s_gu),
+                 _vp(stack.w_dn), _vp(stack.s_dn), E, I, _ACT[act], _vp(out), _vp(ws), wsb, _stream(dev))
+    return out
+
+
 class SparseMoE(nn.Module):
     """Drop-in for fni8serve.models.moe.SparseMoE (same constructor, same routing)."""
 
@@ -218,11 +260,9 @@ class SparseMoE(nn.Module):
         B, S, H = x.shape
         xf = x.reshape(-1, H)
         router_logits = F.linear(xf.float(), self.gate.float())  # moe.py:65, same op
-        topi, topw = route(router_logits, self.top_k, scoring=self.scoring_func, sel_bias=self.e_score_bias,
-                           num_expert_groups=self.num_expert_groups, topk_group=self.topk_group,
-                           norm_topk_prob=self.norm_topk_prob, scaling=self.routed_scaling_factor,
-                           weight_dtype=x.dtype)
-        out = experts(xf, topi, topw, self.stack, self.act)
+        out = layer(xf, router_logits, self.stack, self.top_k, scoring=self.scoring_func, sel_bias=self.e_score_bias,
+                    num_expert_groups=self.num_expert_groups, topk_group=self.topk_group,
+                    norm_topk_prob=self.norm_topk_prob, scaling=self.routed_scaling_factor, act=self.act)
         if self.shared is not None:
             gu, dn = self.shared
             shared_out = linear(act_and_mul(linear(xf, gu), self.act), dn)

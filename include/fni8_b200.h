@@ -362,6 +362,19 @@ FNI8_API int fni8_moe_experts_w8a8(const void* x, int dtype, int64_t T, int64_t 
                           const float* s_dn, int64_t E, int64_t I, int act, void* out, void* workspace,
                           size_t workspace_bytes, void* stream);
 
+/* The same from the router's logits [T, E] on: fni8_moe_route (weights rounded to dtype), then
+ * fni8_moe_experts_w8a8 (SparseMoE.forward without the shared expert,
+ * fni8serve/models/moe.py:62-105); the routing is not returned. Up to 16 tokens, where the
+ * rows fit into shared memory, run in two kernels that read each active expert's weights
+ * once (fni8_moe_experts_w8a8 likewise); the results are those of the separate calls, bit for
+ * bit, for any T. E <= 512. */
+FNI8_API size_t fni8_moe_layer_workspace_bytes(int64_t T, int64_t H, int64_t top_k, int64_t E, int64_t I);
+FNI8_API int fni8_moe_layer_w8a8(const void* x, int dtype, int64_t T, int64_t H, const float* logits, int64_t top_k,
+                                 int scoring, const float* sel_bias, int64_t n_groups, int64_t topk_group,
+                                 int norm_topk, float scaling, const int8_t* w_gu, const float* s_gu,
+                                 const int8_t* w_dn, const float* s_dn, int64_t E, int64_t I, int act, void* out,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------ expert-parallel exchange
  * New capability: the reference runs every expert on one GPU (fni8serve/models/moe.py:99-105)
  * and forbids tensor parallelism (fni8serve/config.py:40-45). One process per GPU; rows move
