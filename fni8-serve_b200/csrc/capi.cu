@@ -238,7 +238,7 @@ extern "C" int fni8_device_status(int* code_out) {
   if (code_out == nullptr) return fail(FNI8_ERR_INVALID, "null code_out");
   cudaError_t e = cudaDeviceSynchronize();
   if (e != cudaSuccess) return cuda_status(e, "cudaDeviceSynchronize");
-  int codes[7] = {0, 0, 0, 0, 0, 0, 0};
+  int codes[8] = {};
   if (int s = tile_status_read_and_clear(&codes[0])) return s;
   if (int s = stream_status_read_and_clear(&codes[1])) return s;
   if (int s = splitk_status_read_and_clear(&codes[2])) return s;
@@ -246,6 +246,7 @@ extern "C" int fni8_device_status(int* code_out) {
   if (int s = ep_status_read_and_clear(&codes[4])) return s;
   if (int s = fp4_status_read_and_clear(&codes[5])) return s;
   if (int s = few_status_read_and_clear(&codes[6])) return s;
+  if (int s = fp4s_status_read_and_clear(&codes[7])) return s;
   *code_out = 0;
   for (int v : codes)
     if (*code_out == 0) *code_out = v;

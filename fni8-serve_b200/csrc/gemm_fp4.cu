@@ -448,10 +448,12 @@ int launch_tile(const Fp4Gemm& g, cudaStream_t st) {
 
 template <int FMT>
 int pick_tile(const Fp4Gemm& g, cudaStream_t st) {
+  if (g.M > 128) return launch_tile<FMT, 256, true>(g, st);
   return launch_tile<FMT, 128, false>(g, st);
 }
 
 int run_gemm(const Fp4Gemm& g, cudaStream_t st) {
+  if (g.M <= 128) return fp4_splitk(g, st);
   if (g.format == FNI8_MXFP4) return pick_tile<FNI8_MXFP4>(g, st);
   return pick_tile<FNI8_NVFP4>(g, st);
 }

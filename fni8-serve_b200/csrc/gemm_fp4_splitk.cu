@@ -1,0 +1,353 @@
+// Decode GEMM of 4-bit floating point operands (1 to 128 tokens): every SM streams weights.
+//
+//   acc^T[n, m] = sum_k w[n,k] sw[n,k/g] a[m,k] sa[m,k/g]   (tcgen05.mma kind::mxf4 / mxf4nvf4)
+//   out[m, n]   = dtype(acc * ra[m] * rw[n] (+ bias[n]))
+//
+// Bound: HBM, N K (1/2 + 1/g) bytes of weights read once. As in gemm_splitk.cu the operands
+// are swapped (128 weight rows = MMA M, NT tokens = MMA N) and a cluster of S CTAs splits the
+// K range of a weight tile, S chosen so that the grid fills the GPU once; weights are loaded
+// before the wait for the quantiser. Here the S partial accumulators meet in shared memory:
+// CTA r owns 128 / S weight rows, every CTA stores the other ranks' rows of its accumulator
+// into their landing areas (distributed shared memory), and the owner adds the S parts in
+// rank order, so the result does not depend on timing and there is no workspace.
+#include <mutex>
+
+#include "fp4_common.cuh"
+#include "gemm_internal.h"
+
+namespace fni8b {
+namespace fp4s {
+
+using namespace fp4;
+
+constexpr int kThreads = 192;
+constexpr int kMaxStages = 8;
+
+static __device__ int g_status;
+enum : int { kCodeProducer = 0x711, kCodeMma = 0x712, kCodeEpilogue = 0x713, kCodeDrain = 0x714 };
+
+struct Epi {
+  const float* a_rs;
+  const float* w_rs;
+  const void* bias;
+  void* out;
+  int bf16;
+};
+
+template <int FMT, int NT>
+struct Cfg {
+  static constexpr int TILES = Fmt<FMT>::kStageTiles;
+  static constexpr int W_BYTES = 128 * 128;
+  static constexpr int X_BYTES = NT * 128;
+  static constexpr int SF_BYTES = TILES * 512;
+  static constexpr int STAGE = W_BYTES + X_BYTES + 2 * SF_BYTES;
+  static constexpr int ACC_COLS = NT;
+  static constexpr int SF_COLS = 8 * TILES;  // weights', then tokens' scales of a stage
+  static constexpr int COLS = ACC_COLS + 2 * SF_COLS;
+  static constexpr int TMEM_COLS = COLS <= 64 ? 64 : COLS <= 128 ? 128 : 256;
+  static_assert(STAGE % 1024 == 0, "stages keep the 1024-byte alignment of the swizzle");
+};
+
+// weight rows that rank r of S owns: [r R, min(128, (r + 1) R))
+__host__ __device__ __forceinline__ int owned_rows(int S) { return (128 + S - 1) / S; }
+
+template <int FMT>
+__device__ __forceinline__ void put(const Epi& epi, float v, int m, int n, int N) {
+  if constexpr (FMT == FNI8_NVFP4) v = __fmul_rn(__fmul_rn(v, __ldg(epi.a_rs + m)), __ldg(epi.w_rs + n));
+  const int64_t at = static_cast<int64_t>(m) * N + n;
+  if (epi.bf16) {
+    if (epi.bias != nullptr) v = __fadd_rn(v, __bfloat162float(static_cast<const __nv_bfloat16*>(epi.bias)[n]));
+    static_cast<__nv_bfloat16*>(epi.out)[at] = __float2bfloat16_rn(v);
+  } else {
+    if (epi.bias != nullptr) v = __fadd_rn(v, __half2float(static_cast<const __half*>(epi.bias)[n]));
+    static_cast<__half*>(epi.out)[at] = __float2half_rn(v);
+  }
+}
+
+template <int FMT, int NT>
+__global__ void __launch_bounds__(kThreads, 2)
+    fp4_splitk_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                      const __grid_constant__ CUtensorMap tmSW, const __grid_constant__ CUtensorMap tmSX, Epi epi, int M,
+                      int N, int Kp, int ktiles, int stages) {
+  using C = Cfg<FMT, NT>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + stages * C::STAGE);
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* tfull = empty + kMaxStages;
+  uint64_t* drain = tfull + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  float* land = reinterpret_cast<float*>(smem + stages * C::STAGE + 256);  // [S][M][R]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_ctarank()), S = static_cast<int>(cluster_nctarank());
+  const int tile = static_cast<int>(blockIdx.x) / S;
+  const int kb = (Kp + 255) / 256;
+  const int kbeg = static_cast<int>(static_cast<int64_t>(rank) * kb / S);
+  const int nk = static_cast<int>(static_cast<int64_t>(rank + 1) * kb / S) - kbeg;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(tfull, 1);
+    mbar_init(drain, 1);
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::TMEM_COLS);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  // the peers have started before anything is stored into their shared memory
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+
+  int okt = 0;
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      tma_prefetch_desc(&tmW);
+      tma_prefetch_desc(&tmX);
+      tma_prefetch_desc(&tmSW);
+      tma_prefetch_desc(&tmSX);
+      auto load_w = [&](int s, int k) {
+        uint8_t* dst = smem + s * C::STAGE;
+        mbar_arrive_expect_tx(&full[s], C::STAGE);
+        tma_load_2d(&tmW, &full[s], dst, k * 128, tile * 128);
+        tma_load_2d(&tmSW, &full[s], dst + C::W_BYTES + C::X_BYTES, 0, (tile * ktiles + k * C::TILES) * 4);
+      };
+      auto load_x = [&](int s, int k) {
+        uint8_t* dst = smem + s * C::STAGE;
+        tma_load_2d(&tmX, &full[s], dst + C::W_BYTES, k * 128, 0);
+        tma_load_2d(&tmSX, &full[s], dst + C::W_BYTES + C::X_BYTES + C::SF_BYTES, 0, k * C::TILES * 4);
+      };
+      const int pre = nk < stages ? nk : stages;
+      for (int i = 0; i < pre; ++i) load_w(i, kbeg + i);
+      pdl_wait();
+      for (int i = 0; i < pre; ++i) load_x(i, kbeg + i);
+      int stage = pre % stages, issued = pre;
+      uint32_t ph = pre == stages ? 1u : 0u, armed = 0;
+      for (int i = pre; i < nk; ++i) {
+        if (!mbar_wait(&empty[stage], ph ^ 1u, &g_status, kCodeProducer)) break;
+        load_w(stage, kbeg + i);
+        load_x(stage, kbeg + i);
+        armed = (armed & ~(1u << stage)) | (ph << stage);
+        ++issued;
+        if (++stage == stages) {
+          stage = 0;
+          ph ^= 1u;
+        }
+      }
+      const int pending = issued < stages ? issued : stages;
+      for (int i = 0; i < pending; ++i) {
+        const int s = (stage - 1 - i + 2 * stages) % stages;
+        mbar_wait(&full[s], (armed >> s) & 1u, &g_status, kCodeDrain);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int i = 0; i < nk; ++i) {
+        if (!mbar_wait(&full[stage], ph, &g_status, kCodeMma)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint8_t* sw = smem + stage * C::STAGE;
+        const uint8_t* sf = sw + C::W_BYTES + C::X_BYTES;
+        const uint32_t ta = tmem_base + C::ACC_COLS + static_cast<uint32_t>((i & 1) * C::SF_COLS);
+        const uint32_t tb = ta + 4 * C::TILES;
+#pragma unroll
+        for (int t = 0; t < C::TILES; ++t) {
+          copy_scales<false>(ta + t * 4, scale_desc(smem_u32(sf + t * 512)));
+          copy_scales<false>(tb + t * 4, scale_desc(smem_u32(sf + C::SF_BYTES + t * 512)));
+        }
+        const int steps = min(4, (Kp - (kbeg + i) * 256 + 63) / 64);
+        stage_mmas<FMT, false, 128, NT>(tmem_base, sw, sw + C::W_BYTES, ta, tb, steps, i == 0);
+        umma_commit(&empty[stage]);
+        if (++stage == stages) {
+          stage = 0;
+          ph ^= 1u;
+        }
+      }
+      if (ok) umma_commit(tfull);
+      umma_commit(drain);
+      mbar_wait(drain, 0, &g_status, kCodeDrain);
+    }
+  } else {
+    pdl_wait();
+    if (lane == 0) okt = mbar_wait(tfull, 0, &g_status, kCodeEpilogue) ? 1 : 0;
+    okt = __shfl_sync(0xffffffffu, okt, 0);
+    tc_fence_after();
+  }
+  __syncwarp();
+  pdl_wait();  // every thread may write out below
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+
+  const int row = (warp & 3) * 32 + lane;  // epilogue warps 2-5 read the TMEM lanes of quarters 2, 3, 0, 1
+  const uint32_t taddr = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+  const int R = owned_rows(S);
+  if (warp >= 2 && okt) {
+    const int n = tile * 128 + row;
+    const int owner = row / R;
+    const uint32_t dst = mapa_shared(smem_u32(land), static_cast<uint32_t>(owner)) +
+                         static_cast<uint32_t>((rank * M * R + row - owner * R) * 4);
+#pragma unroll 1
+    for (int c0 = 0; c0 < M; c0 += 16) {
+      uint32_t r[16];
+      tmem_ld16(taddr + static_cast<uint32_t>(c0), r);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        if (c0 + j < M) {
+          if (S == 1) {
+            if (n < N) put<FMT>(epi, __uint_as_float(r[j]), c0 + j, n, N);
+          } else {
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst + static_cast<uint32_t>((c0 + j) * R * 4)), "r"(r[j])
+                         : "memory");
+          }
+        }
+      }
+    }
+    tc_fence_before();
+  }
+  if (S > 1) {
+    __syncwarp();
+    cluster_sync_all();
+    pdl_launch_dependents();
+    const int rows = min(R, 128 - rank * R);
+    const int n0 = tile * 128 + rank * R;
+    for (int i = threadIdx.x; i < M * R; i += kThreads) {
+      const int m = i / R, r = i - m * R;
+      if (r < rows && n0 + r < N) {
+        float v = land[i];
+        for (int s = 1; s < S; ++s) v = __fadd_rn(v, land[s * M * R + i]);
+        put<FMT>(epi, v, m, n0 + r, N);
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, C::TMEM_COLS);
+  }
+}
+
+}  // namespace fp4s
+}  // namespace fni8b
+
+namespace fni8h {
+
+using namespace fni8b;
+
+int fp4s_status_read_and_clear(int* code) {
+  int v = 0, z = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, fp4s::g_status, sizeof(int));
+  if (e != cudaSuccess) return cuda_status(e, "read fp4 split-K watchdog");
+  e = cudaMemcpyToSymbol(fp4s::g_status, &z, sizeof(int));
+  if (e != cudaSuccess) return cuda_status(e, "clear fp4 split-K watchdog");
+  *code = v;
+  return FNI8_OK;
+}
+
+namespace {
+
+// Clusters of S CTAs with `smem` bytes that are resident at once, remembered per device.
+int resident_clusters(int smem, int S) {
+  struct Entry { int dev, smem, S, n; };
+  static Entry cache[64];
+  static int used = 0;
+  static std::mutex mu;
+  std::lock_guard<std::mutex> lock(mu);
+  const int dev = current_device();
+  for (int i = 0; i < used; ++i)
+    if (cache[i].dev == dev && cache[i].smem == smem && cache[i].S == S) return cache[i].n;
+  const int n = max_active_clusters(fp4s::kThreads, smem, S);
+  if (n >= 0 && used < 64) cache[used++] = Entry{dev, smem, S, n};
+  return n;
+}
+
+template <int FMT, int NT>
+int launch_splitk(const Fp4Gemm& g, cudaStream_t st) {
+  using C = fp4s::Cfg<FMT, NT>;
+  auto kern = fp4s::fp4_splitk_kernel<FMT, NT>;
+  static std::atomic<bool> configured[kMaxDevices] = {};
+  const int dev = current_device();
+  if (dev < 0 || dev >= kMaxDevices) return fail(FNI8_ERR_CUDA, "no current CUDA device");
+  if (!configured[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(fp4 split-K)");
+    configured[dev] = true;
+  }
+  const int tiles = (int)((g.N + 127) / 128), kb = (int)((fp4::padded_k(g.K) + 255) / 256);
+  // Ring: half an SM's shared memory (two CTAs per SM) up to 32 tokens, a whole SM's beyond.
+  auto plan = [&](int S, int* stages) {
+    const int land = S > 1 ? S * (int)g.M * fp4s::owned_rows(S) * 4 : 0;
+    const int fixed = 1024 + 256 + land;
+    const int per = (kb + S - 1) / S;
+    int n = ((NT <= 32 ? 113 : 225) * 1024 - fixed) / C::STAGE;
+    n = n < fp4s::kMaxStages ? n : fp4s::kMaxStages;
+    *stages = n < per ? n : per;
+    return fixed + *stages * C::STAGE;
+  };
+  const int sms = num_sms(dev), slots = NT <= 32 ? 2 * sms : sms;
+  int S = slots / tiles;
+  S = S < 1 ? 1 : S > 8 ? 8 : S;
+  S = S > kb ? kb : S;
+  int stages = 0, smem = plan(S, &stages);
+  while (S > 1) {
+    const int n = resident_clusters(smem, S);
+    if (n < 0 || tiles <= n) break;
+    smem = plan(--S, &stages);
+  }
+  const uint64_t row = (uint64_t)fp4::padded_k(g.K) / 2;
+  CUtensorMap tw, tx, tsw, tsx;
+  if (int s = encode_tmap_2d_i8(&tw, g.w, row, (uint64_t)g.N, row, 128, 128)) return s;
+  if (int s = encode_tmap_2d_i8(&tx, g.a, row, (uint64_t)g.M, row, 128, NT)) return s;
+  if (int s = encode_scale_map(&tsw, g.w_sf, FMT, g.N, g.K, C::TILES)) return s;
+  if (int s = encode_scale_map(&tsx, g.a_sf, FMT, g.M, g.K, C::TILES)) return s;
+  const fp4s::Epi epi{g.a_rs, g.w_rs, g.bias, g.out, g.bf16 ? 1 : 0};
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * S));
+  cfg.blockDim = dim3(fp4s::kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = S;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled();
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tw, tx, tsw, tsx, epi, (int)g.M, (int)g.N,
+                                           (int)fp4::padded_k(g.K), (int)fp4::k_tiles(FMT, g.K), stages);
+  if (e != cudaSuccess) return cuda_status(e, "launch fp4 split-K gemm");
+  return FNI8_OK;
+}
+
+template <int FMT>
+int splitk_any(const Fp4Gemm& g, cudaStream_t st) {
+  if (g.M <= 16) return launch_splitk<FMT, 16>(g, st);
+  if (g.M <= 32) return launch_splitk<FMT, 32>(g, st);
+  if (g.M <= 64) return launch_splitk<FMT, 64>(g, st);
+  return launch_splitk<FMT, 128>(g, st);
+}
+
+}  // namespace
+
+int fp4_splitk(const Fp4Gemm& g, cudaStream_t st) {
+  return g.format == FNI8_MXFP4 ? splitk_any<FNI8_MXFP4>(g, st) : splitk_any<FNI8_NVFP4>(g, st);
+}
+
+}  // namespace fni8h

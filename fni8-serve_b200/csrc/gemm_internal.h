@@ -99,7 +99,10 @@ int fp4_check_rows(const void* x, int dtype, int format, int64_t M, int64_t K, c
 // pad: also zero the scales of the rows behind M in the last tile.
 int fp4_quantize(const void* x, int dtype, int format, int64_t M, int64_t K, bool pad, uint8_t* q, uint8_t* sf,
                  float* row_scale, cudaStream_t st);
+// The swap-AB split-K kernel for M <= 128 (gemm_fp4_splitk.cu).
+int fp4_splitk(const Fp4Gemm& g, cudaStream_t st);
 int fp4_status_read_and_clear(int* code);
+int fp4s_status_read_and_clear(int* code);
 
 // The routed-expert layer for a few tokens in two kernels (moe_few.cu). logits null: the
 // routing topi / topw is given. h: scratch [T k, I] of the activations' type, 16-byte aligned,
