@@ -87,12 +87,31 @@ __device__ __forceinline__ void umma_fp4(uint32_t d, uint64_t adesc, uint64_t bd
 }
 #undef FNI8_MMA_FP4
 
-// The 256-value stage's MMAs: `steps` (1 to 4) of 64 values each. sa, sb: the operands'
-// stage (128-byte swizzle), ta, tb: the tensor-memory columns of their scales.
+// A 256-value stage's scale tiles from shared memory (sfa; sfb, the tiles of B's second 128
+// rows behind all of the first's) to the tensor-memory columns ta and tb. Copies and MMAs of
+// a thread execute in order: a copy needs no wait before the MMA that reads it, nor after
+// the one that read its columns before. A copy takes 45 cycles whatever its size (measured
+// on B200) and runs beside the last two MMAs before it, or beside nothing.
+template <int FMT, bool PAIR, int N>
+__device__ __forceinline__ void stage_scales(const uint8_t* sfa, const uint8_t* sfb, uint32_t ta, uint32_t tb) {
+  constexpr int kTiles = Fmt<FMT>::kStageTiles;
+  constexpr int kRowTiles = (N + 127) / 128;  // of B
+  const uint64_t da = scale_desc(smem_u32(sfa)), db = scale_desc(smem_u32(sfb));
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i) {
+    copy_scales<PAIR>(ta + i * 4, da + static_cast<uint64_t>(i * 512 >> 4));
+#pragma unroll
+    for (int j = 0; j < kRowTiles; ++j)
+      copy_scales<PAIR>(tb + (i * kRowTiles + j) * 4, db + static_cast<uint64_t>((j * kTiles + i) * 512 >> 4));
+  }
+}
+
+// The stage's MMAs: `steps` (1 to 4) of 64 values each. sa, sb: the operands' stage (128-byte
+// swizzle).
 template <int FMT, bool PAIR, int M, int N>
 __device__ __forceinline__ void stage_mmas(uint32_t d, const void* sa, const void* sb, uint32_t ta, uint32_t tb,
                                            int steps, bool first) {
-  constexpr int kBCols = (N + 127) / 128 * 4;  // columns of one tile column of B's scales
+  constexpr int kRowTiles = (N + 127) / 128;
   const uint64_t adesc = sw128_kmajor_desc(smem_u32(sa)), bdesc = sw128_kmajor_desc(smem_u32(sb));
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk) {
@@ -100,7 +119,7 @@ __device__ __forceinline__ void stage_mmas(uint32_t d, const void* sa, const voi
       const int tile = FMT == FNI8_MXFP4 ? kk >> 1 : kk;
       const uint32_t idesc = idesc_fp4(FMT, M, N, FMT == FNI8_MXFP4 ? (kk & 1) * 2 : 0);
       umma_fp4<FMT, PAIR>(d, adesc + static_cast<uint64_t>(kk * 2), bdesc + static_cast<uint64_t>(kk * 2), idesc,
-                          ta + static_cast<uint32_t>(tile * 4), tb + static_cast<uint32_t>(tile * kBCols),
+                          ta + static_cast<uint32_t>(tile * 4), tb + static_cast<uint32_t>(tile * kRowTiles * 4),
                           (kk != 0 || !first) ? 1u : 0u);
     }
   }

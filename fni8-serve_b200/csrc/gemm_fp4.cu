@@ -9,9 +9,17 @@
 // Structure of the int8 tile kernel (gemm_tile.cu): one persistent CTA per SM, a TMA warp,
 // an MMA warp, eight epilogue warps. A stage is 128 bytes of K (256 values) of 128 rows of a
 // and BN rows of w with the 128-byte swizzle, plus their scale tiles as they lie in memory
-// (512 bytes each, no swizzle); the MMA thread copies the scale tiles into tensor memory
-// with tcgen05.cp before the stage's four MMAs. Copies and MMAs of one thread execute in
-// order, so a stage's scales need no wait; two sets of tensor-memory columns alternate.
+// (512 bytes each, no swizzle); tcgen05.cp brings those into tensor memory.
+//
+// What bounds it: as the int8 kernel, the feed of shared memory from L2 (about 45 B/clk of an
+// SM). The copies must not come on top of that. Measured on B200: one takes 45 cycles of the
+// tensor pipe whatever its shape, so 12 of them (nvfp4, 256 columns) 540, beside 512 for the
+// stage's MMAs; issued by the MMA's thread they overlap neither the MMAs before its last
+// commit nor those behind them (8192 x 4096 x 16384 nvfp4: 358 us, 189 without the copies).
+// From another thread they leave the MMAs at 514 cycles a stage, but a batch then takes some
+// 1400 cycles to complete. So an eleventh warp issues them, and the scales run ahead: their
+// ring is kLead stages deeper than the operands', their tiles are loaded before the
+// operands of earlier stages, and SETS sets of tensor-memory columns take turns.
 #include "fp4_common.cuh"
 #include "gemm_internal.h"
 
@@ -22,12 +30,13 @@ constexpr int BM = 128;
 constexpr int BK = 128;  // bytes of K per stage: 256 values
 constexpr int kEpiWarps = 8;
 constexpr int kEpiThreads = 32 * kEpiWarps;
-constexpr int kTileThreads = 64 + kEpiThreads;
+constexpr int kTileThreads = 64 + kEpiThreads + 32;
+constexpr int kLead = 2;  // stages that the scales run ahead of their operands
 constexpr int kBand = 16;  // m-tiles per band of the tile order: a wave reuses its rows and columns from L2
 
 static __device__ int g_status;
 
-enum : int { kCodeProducer = 0x701, kCodeMma = 0x702, kCodeEpilogue = 0x703, kCodeDrain = 0x704 };
+enum : int { kCodeProducer = 0x701, kCodeMma = 0x702, kCodeEpilogue = 0x703, kCodeDrain = 0x704, kCodeScales = 0x705 };
 
 struct Epi {
   const float* a_rs;  // [M] or null (mxfp4)
@@ -47,18 +56,24 @@ struct Cfg {
   static constexpr int B_BYTES = BNL * BK;
   static constexpr int SFA_BYTES = TILES * 512;
   static constexpr int SFB_BYTES = BN / 128 * TILES * 512;  // of all BN columns, in both CTAs of a pair
-  static constexpr int STAGE = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
+  static constexpr int STAGE = A_BYTES + B_BYTES;
+  static constexpr int SF = SFA_BYTES + SFB_BYTES;
   static constexpr int STG_BUF = 32 * 32 * 2;  // one output slab of an epilogue warp
-  static constexpr int FIXED = 1024 + 1024 + kEpiWarps * STG_BUF + 2 * BN * 4;
-  static constexpr int STAGES = (227 * 1024 - FIXED) / STAGE;
-  static constexpr int STG_OFF = STAGES * STAGE + 1024;  // barriers in between; 1024-aligned
-  static constexpr int SMEM = FIXED + STAGES * STAGE;
-  // accumulators in columns [0, 256), then two sets of scale columns
+  static constexpr int FIXED = 1024 + 1024 + kEpiWarps * STG_BUF + 2 * BN * 4 + kLead * SF;
+  static constexpr int STAGES = (227 * 1024 - FIXED) / (STAGE + SF);
+  static constexpr int SLOTS = STAGES + kLead;  // scale ring
+  static constexpr int SF_OFF = STAGES * STAGE;
+  static constexpr int BAR_OFF = SF_OFF + SLOTS * SF;
+  static constexpr int STG_OFF = BAR_OFF + 1024;  // 1024-aligned
+  static constexpr int SMEM = FIXED + STAGES * (STAGE + SF);
+  // accumulators in columns [0, 256), then the sets of scale columns
   static constexpr int NACC = 256 / BN;
   static constexpr int SFA_COLS = TILES * 4;
   static constexpr int SF_COLS = SFA_COLS + BN / 128 * TILES * 4;
-  static_assert(256 + 2 * SF_COLS <= 512, "tensor memory");
+  static constexpr int SETS = 4;
+  static_assert(256 + SETS * SF_COLS <= 512 && SETS < STAGES, "tensor memory");
   static_assert(STAGES >= 3 && STAGES <= 8, "ring");
+  static_assert(STG_OFF % 1024 == 0, "the store's swizzle follows address bits");
 };
 
 template <int BMT>
@@ -126,12 +141,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   using C = Cfg<FMT, BN, PAIR>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
   uint64_t* empty = full + C::STAGES;
-  uint64_t* tfull = empty + C::STAGES;
+  uint64_t* sfull = empty + C::STAGES;
+  uint64_t* sready = sfull + C::SLOTS;
+  uint64_t* tfull = sready + C::SETS;
   uint64_t* tempty = tfull + 2;
   uint64_t* drain = tempty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   uint8_t* stg = smem + C::STG_OFF;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -144,11 +161,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
+    for (int s = 0; s < C::SLOTS; ++s) mbar_init(&sfull[s], 1);
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull[b], 1);
       mbar_init(&tempty[b], PAIR ? 2 * kEpiWarps : kEpiWarps);
     }
+    for (int s = 0; s < C::SETS; ++s) mbar_init(&sready[s], 1);
     mbar_init(drain, 1);
+    mbar_init(drain + 1, 1);
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -179,52 +199,86 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       tma_prefetch_desc(&tmB);
       tma_prefetch_desc(&tmSA);
       tma_prefetch_desc(&tmSB);
-      constexpr uint32_t kTx = PAIR ? 2 * C::STAGE : C::STAGE;
-      auto load = [&](const CUtensorMap* map, int s, int off, int cx, int cy) {
-        uint8_t* dst = smem + s * C::STAGE + off;
-        if constexpr (PAIR) tma_load_2d_pair(map, mapa_shared(smem_u32(&full[s]), 0), dst, cx, cy);
-        else tma_load_2d(map, &full[s], dst, cx, cy);
+      constexpr int kCtas = PAIR ? 2 : 1;  // a pair's loads complete on the even CTA's barriers
+      auto load = [&](const CUtensorMap* map, uint64_t* bar, int off, int cx, int cy) {
+        if constexpr (PAIR) tma_load_2d_pair(map, mapa_shared(smem_u32(bar), 0), smem + off, cx, cy);
+        else tma_load_2d(map, bar, smem + off, cx, cy);
       };
-      auto load_a = [&](int s, int m_blk, int k) {
-        const int rt = PAIR ? 2 * m_blk + static_cast<int>(half) : m_blk;  // this CTA's 128 rows
-        load(&tmA, s, 0, k * BK, rt * BM);
-        load(&tmSA, s, C::A_BYTES + C::B_BYTES, 0, (rt * ktiles + k * C::TILES) * 4);
+      // this CTA's 128 rows of an m-tile
+      auto row_tile = [&](int m_blk) { return PAIR ? 2 * m_blk + static_cast<int>(half) : m_blk; };
+      // (tile, stage of it) that a load is for; two of them walk the same sequence
+      struct Pos {
+        int t, k, mb, nb;
       };
-      auto load_b = [&](int s, int n_blk, int k) {
-        load(&tmB, s, C::A_BYTES, k * BK, n_blk * BN + static_cast<int>(half) * C::BNL);
-#pragma unroll
-        for (int i = 0; i < BN / 128; ++i)
-          load(&tmSB, s, C::A_BYTES + C::B_BYTES + C::SFA_BYTES + i * C::TILES * 512, 0,
-               ((n_blk * (BN / 128) + i) * ktiles + k * C::TILES) * 4);
+      auto start = [&](Pos& p) {
+        p = Pos{t0, 0, 0, 0};
+        if (p.t < total) tile_at<C::BMT>(p.t, m_tiles, n_tiles, p.mb, p.nb);
       };
-      int stage = 0, issued = 0, t = t0, k = 0, mb = 0, nb = 0;
-      uint32_t ph = 0, armed = 0;
-      if (t < total) tile_at<C::BMT>(t, m_tiles, n_tiles, mb, nb);
-      auto advance = [&]() {
-        if (++k == kb) {
-          k = 0;
-          t += tstep;
-          if (t < total) tile_at<C::BMT>(t, m_tiles, n_tiles, mb, nb);
+      auto advance = [&](Pos& p) {
+        if (++p.k == kb) {
+          p.k = 0;
+          p.t += tstep;
+          if (p.t < total) tile_at<C::BMT>(p.t, m_tiles, n_tiles, p.mb, p.nb);
         }
       };
-      int pre_m[C::STAGES], pre_k[C::STAGES];
-      int pre = 0;
-      for (; pre < C::STAGES && t < total; ++pre, advance()) {
-        if (half == 0) mbar_arrive_expect_tx(&full[pre], kTx);
-        load_b(pre, nb, k);
-        pre_m[pre] = mb;
-        pre_k[pre] = k;
+      auto load_a = [&](int s, const Pos& p) {
+        load(&tmA, &full[s], s * C::STAGE, p.k * BK, row_tile(p.mb) * BM);
+      };
+      auto load_b = [&](int s, const Pos& p) {
+        if (half == 0) mbar_arrive_expect_tx(&full[s], kCtas * C::STAGE);
+        load(&tmB, &full[s], s * C::STAGE + C::A_BYTES, p.k * BK, p.nb * BN + static_cast<int>(half) * C::BNL);
+      };
+      auto load_sa = [&](int u, const Pos& p) {
+        load(&tmSA, &sfull[u], C::SF_OFF + u * C::SF, 0, (row_tile(p.mb) * ktiles + p.k * C::TILES) * 4);
+      };
+      auto load_sb = [&](int u, const Pos& p) {
+        if (half == 0) mbar_arrive_expect_tx(&sfull[u], kCtas * C::SF);
+#pragma unroll
+        for (int i = 0; i < BN / 128; ++i)
+          load(&tmSB, &sfull[u], C::SF_OFF + u * C::SF + C::SFA_BYTES + i * C::TILES * 512, 0,
+               ((p.nb * (BN / 128) + i) * ktiles + p.k * C::TILES) * 4);
+      };
+      Pos x, y;  // next operand stage, next scale slot (kLead ahead)
+      start(x);
+      start(y);
+      int slot = 0, stage = 0, issued = 0;
+      uint32_t ph = 0, armed = 0, slot_ph = 0, slot_armed = 0;
+      auto next_slot = [&]() {
+        slot_armed = (slot_armed & ~(1u << slot)) | (slot_ph << slot);
+        advance(y);
+        if (++slot == C::SLOTS) {
+          slot = 0;
+          slot_ph ^= 1u;
+        }
+      };
+      // the weights' part of the first ring does not depend on the quantiser
+      Pos first_x[C::STAGES], first_y[C::SLOTS];
+      int nx = 0, ny = 0;
+      for (; ny < C::SLOTS && y.t < total; ++ny) {
+        load_sb(slot, y);
+        first_y[ny] = y;
+        next_slot();
+      }
+      for (; nx < C::STAGES && x.t < total; ++nx, advance(x)) {
+        load_b(nx, x);
+        first_x[nx] = x;
       }
       pdl_wait();
-      for (int i = 0; i < pre; ++i) load_a(i, pre_m[i], pre_k[i]);
-      issued = pre;
-      stage = pre % C::STAGES;
-      ph = pre == C::STAGES ? 1u : 0u;
-      for (; t < total; advance()) {
+      for (int i = 0; i < ny; ++i) load_sa(i, first_y[i]);
+      for (int i = 0; i < nx; ++i) load_a(i, first_x[i]);
+      issued = nx;
+      stage = nx % C::STAGES;
+      ph = nx == C::STAGES ? 1u : 0u;
+      for (; x.t < total; advance(x)) {
+        // frees the operands of the stage, and the scale slot behind it
         if (!mbar_wait(&empty[stage], ph ^ 1u, &g_status, kCodeProducer)) break;
-        if (half == 0) mbar_arrive_expect_tx(&full[stage], kTx);
-        load_a(stage, mb, k);
-        load_b(stage, nb, k);
+        if (y.t < total) {
+          load_sb(slot, y);
+          load_sa(slot, y);
+          next_slot();
+        }
+        load_b(stage, x);
+        load_a(stage, x);
         armed = (armed & ~(1u << stage)) | (ph << stage);
         ++issued;
         if (++stage == C::STAGES) {
@@ -233,51 +287,47 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
       }
       pdl_launch_dependents();
-      // every load lands before the CTA may exit (the odd CTA of a pair sees its loads land
-      // through the release of the stage)
+      // Every load lands before the CTA may exit (normally all have: the MMAs consumed them).
+      // The odd CTA of a pair sees its loads land through the release of their stages.
       uint64_t* done = half == 0 ? full : empty;
       const int pending = issued < C::STAGES ? issued : C::STAGES;
       for (int i = 0; i < pending; ++i) {
         const int s = (stage - 1 - i + 2 * C::STAGES) % C::STAGES;
         mbar_wait(&done[s], (armed >> s) & 1u, &g_status, kCodeDrain);
       }
+      const int used = slot_ph != 0u || slot_armed != 0u ? C::SLOTS : slot;
+      if (half == 0)
+        for (int u = 0; u < used; ++u) mbar_wait(&sfull[u], (slot_armed >> u) & 1u, &g_status, kCodeDrain);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     if (lane == 0 && half == 0) {
       int stage = 0, acc = 0, set = 0;
-      uint32_t ph = 0, aph = 0;
+      uint32_t ph = 0, aph = 0, sph = 0;
       bool ok = true;
       for (int t = t0; t < total && ok; t += tstep) {
         if (!mbar_wait(&tempty[acc], aph ^ 1u, &g_status, kCodeMma)) break;
         tc_fence_after();
         const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
         for (int k = 0; k < kb; ++k) {
-          if (!mbar_wait(&full[stage], ph, &g_status, kCodeMma)) {
+          if (!mbar_wait(&sready[set], sph, &g_status, kCodeMma) || !mbar_wait(&full[stage], ph, &g_status, kCodeMma)) {
             ok = false;
             break;
           }
           tc_fence_after();
           const uint8_t* sa = smem + stage * C::STAGE;
-          const uint8_t* sfa = sa + C::A_BYTES + C::B_BYTES;
-          const uint32_t ta = tmem_base + 256u + static_cast<uint32_t>(set * C::SF_COLS);
-          const uint32_t tb = ta + C::SFA_COLS;
-#pragma unroll
-          for (int i = 0; i < C::TILES; ++i) {
-            copy_scales<PAIR>(ta + i * 4, scale_desc(smem_u32(sfa + i * 512)));
-#pragma unroll
-            for (int j = 0; j < BN / 128; ++j)
-              copy_scales<PAIR>(tb + (i * (BN / 128) + j) * 4,
-                                scale_desc(smem_u32(sfa + C::SFA_BYTES + (j * C::TILES + i) * 512)));
-          }
           const int steps = min(4, (Kp - k * 256 + 63) / 64);
-          stage_mmas<FMT, PAIR, C::BMT, BN>(d, sa, sa + C::A_BYTES, ta, tb, steps, k == 0);
+          const uint32_t sc = tmem_base + 256u + static_cast<uint32_t>(set * C::SF_COLS);
+          stage_mmas<FMT, PAIR, C::BMT, BN>(d, sa, sa + C::A_BYTES, sc, sc + C::SFA_COLS, steps, k == 0);
           if constexpr (PAIR) umma_commit_pair_to(&empty[stage], 3);
           else umma_commit(&empty[stage]);
-          set ^= 1;
           if (++stage == C::STAGES) {
             stage = 0;
             ph ^= 1u;
+          }
+          if (++set == C::SETS) {
+            set = 0;
+            sph ^= 1u;
           }
         }
         if (!ok) break;
@@ -291,6 +341,39 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if constexpr (PAIR) umma_commit_pair(drain);
       else umma_commit(drain);
       mbar_wait(drain, 0, &g_status, kCodeDrain);
+    }
+    __syncwarp();
+  } else if (warp == 2 + kEpiWarps) {
+    // ------------------------------------------------------------ scales into tensor memory
+    if (lane == 0 && half == 0) {
+      int slot = 0, set = 0, freed = 0;  // freed: the operand stage whose release frees the set
+      uint32_t ph = 0, fph = 0;
+      const int per = t0 < total ? (total - t0 - 1) / tstep + 1 : 0;
+      const int64_t stages = static_cast<int64_t>(per) * kb;
+      for (int64_t j = 0; j < stages; ++j) {
+        if (!mbar_wait(&sfull[slot], ph, &g_status, kCodeScales)) break;
+        if (j >= C::SETS) {
+          if (!mbar_wait(&empty[freed], fph, &g_status, kCodeScales)) break;
+          if (++freed == C::STAGES) {
+            freed = 0;
+            fph ^= 1u;
+          }
+        }
+        tc_fence_after();
+        const uint8_t* sf = smem + C::SF_OFF + slot * C::SF;
+        const uint32_t sc = tmem_base + 256u + static_cast<uint32_t>(set * C::SF_COLS);
+        stage_scales<FMT, PAIR, BN>(sf, sf + C::SFA_BYTES, sc, sc + C::SFA_COLS);
+        if constexpr (PAIR) umma_commit_pair(&sready[set]);
+        else umma_commit(&sready[set]);
+        if (++set == C::SETS) set = 0;
+        if (++slot == C::SLOTS) {
+          slot = 0;
+          ph ^= 1u;
+        }
+      }
+      if constexpr (PAIR) umma_commit_pair(drain + 1);
+      else umma_commit(drain + 1);
+      mbar_wait(drain + 1, 0, &g_status, kCodeDrain);
     }
     __syncwarp();
   } else {

@@ -164,12 +164,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         const uint8_t* sf = sw + C::W_BYTES + C::X_BYTES;
         const uint32_t ta = tmem_base + C::ACC_COLS + static_cast<uint32_t>((i & 1) * C::SF_COLS);
         const uint32_t tb = ta + 4 * C::TILES;
-#pragma unroll
-        for (int t = 0; t < C::TILES; ++t) {
-          copy_scales<false>(ta + t * 4, scale_desc(smem_u32(sf + t * 512)));
-          copy_scales<false>(tb + t * 4, scale_desc(smem_u32(sf + C::SF_BYTES + t * 512)));
-        }
         const int steps = min(4, (Kp - (kbeg + i) * 256 + 63) / 64);
+        stage_scales<FMT, false, NT>(sf, sf + C::SF_BYTES, ta, tb);
         stage_mmas<FMT, false, 128, NT>(tmem_base, sw, sw + C::W_BYTES, ta, tb, steps, i == 0);
         umma_commit(&empty[stage]);
         if (++stage == stages) {
