@@ -87,22 +87,23 @@ __device__ __forceinline__ void umma_fp4(uint32_t d, uint64_t adesc, uint64_t bd
 }
 #undef FNI8_MMA_FP4
 
-// A 256-value stage's scale tiles from shared memory (sfa; sfb, the tiles of B's second 128
-// rows behind all of the first's) to the tensor-memory columns ta and tb. Copies and MMAs of
-// a thread execute in order: a copy needs no wait before the MMA that reads it, nor after
-// the one that read its columns before. A copy takes 45 cycles whatever its size (measured
-// on B200) and runs beside the last two MMAs before it, or beside nothing.
-template <int FMT, bool PAIR, int N>
+// Every PARTS-th (from PART on) of a 256-value stage's scale tiles, from shared memory (sfa;
+// sfb, the tiles of B's second 128 rows behind all of the first's) to the tensor-memory columns
+// ta and tb. Copies and MMAs of one thread execute in order: a copy needs no wait before the
+// MMA that reads it, nor after the one that read its columns before.
+template <int FMT, bool PAIR, int N, int PART = 0, int PARTS = 1>
 __device__ __forceinline__ void stage_scales(const uint8_t* sfa, const uint8_t* sfb, uint32_t ta, uint32_t tb) {
   constexpr int kTiles = Fmt<FMT>::kStageTiles;
   constexpr int kRowTiles = (N + 127) / 128;  // of B
   const uint64_t da = scale_desc(smem_u32(sfa)), db = scale_desc(smem_u32(sfb));
 #pragma unroll
-  for (int i = 0; i < kTiles; ++i) {
-    copy_scales<PAIR>(ta + i * 4, da + static_cast<uint64_t>(i * 512 >> 4));
-#pragma unroll
-    for (int j = 0; j < kRowTiles; ++j)
+  for (int c = PART; c < kTiles * (1 + kRowTiles); c += PARTS) {
+    if (c < kTiles) {
+      copy_scales<PAIR>(ta + c * 4, da + static_cast<uint64_t>(c * 512 >> 4));
+    } else {
+      const int i = (c - kTiles) / kRowTiles, j = (c - kTiles) % kRowTiles;
       copy_scales<PAIR>(tb + (i * kRowTiles + j) * 4, db + static_cast<uint64_t>((j * kTiles + i) * 512 >> 4));
+    }
   }
 }
 

@@ -12,14 +12,15 @@
 // (512 bytes each, no swizzle); tcgen05.cp brings those into tensor memory.
 //
 // What bounds it: as the int8 kernel, the feed of shared memory from L2 (about 45 B/clk of an
-// SM). The copies must not come on top of that. Measured on B200: one takes 45 cycles of the
-// tensor pipe whatever its shape, so 12 of them (nvfp4, 256 columns) 540, beside 512 for the
-// stage's MMAs; issued by the MMA's thread they overlap neither the MMAs before its last
-// commit nor those behind them (8192 x 4096 x 16384 nvfp4: 358 us, 189 without the copies).
-// From another thread they leave the MMAs at 514 cycles a stage, but a batch then takes some
-// 1400 cycles to complete. So an eleventh warp issues them, and the scales run ahead: their
-// ring is kLead stages deeper than the operands', their tiles are loaded before the
-// operands of earlier stages, and SETS sets of tensor-memory columns take turns.
+// SM). The copies must not come on top of that. Measured on B200: one thread issues one in 45
+// cycles, whatever its shape, so the 12 of an nvfp4 stage of 256 columns take 540, its MMAs
+// 512; issued by the MMAs' thread they overlap neither the MMAs before its last commit nor
+// those behind them (8192 x 4096 x 16384: mxfp4 256 us, nvfp4 358, without the copies 183 and
+// 189). From other threads they leave the MMAs at 514 cycles a stage, but a stage's copies then
+// complete some 1400 cycles after their issue. So two more warps issue them (211 and 274 us
+// with one, 209 and 232 with two, 219 and 236 with three), and the scales run ahead: their
+// ring is kLead stages deeper than the operands', their tiles are loaded before the operands
+// of earlier stages, and SETS sets of tensor-memory columns take turns.
 #include "fp4_common.cuh"
 #include "gemm_internal.h"
 
@@ -30,7 +31,8 @@ constexpr int BM = 128;
 constexpr int BK = 128;  // bytes of K per stage: 256 values
 constexpr int kEpiWarps = 8;
 constexpr int kEpiThreads = 32 * kEpiWarps;
-constexpr int kTileThreads = 64 + kEpiThreads + 32;
+constexpr int kScaleWarps = 2;
+constexpr int kTileThreads = 64 + kEpiThreads + 32 * kScaleWarps;
 constexpr int kLead = 2;  // stages that the scales run ahead of their operands
 constexpr int kBand = 16;  // m-tiles per band of the tile order: a wave reuses its rows and columns from L2
 
@@ -148,7 +150,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* tfull = sready + C::SETS;
   uint64_t* tempty = tfull + 2;
   uint64_t* drain = tempty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1 + kScaleWarps);
   uint8_t* stg = smem + C::STG_OFF;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -166,9 +168,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(&tfull[b], 1);
       mbar_init(&tempty[b], PAIR ? 2 * kEpiWarps : kEpiWarps);
     }
-    for (int s = 0; s < C::SETS; ++s) mbar_init(&sready[s], 1);
+    for (int s = 0; s < C::SETS; ++s) mbar_init(&sready[s], kScaleWarps);
     mbar_init(drain, 1);
-    mbar_init(drain + 1, 1);
+    for (int s = 0; s < kScaleWarps; ++s) mbar_init(drain + 1 + s, 1);
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -343,9 +345,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_wait(drain, 0, &g_status, kCodeDrain);
     }
     __syncwarp();
-  } else if (warp == 2 + kEpiWarps) {
+  } else if (warp >= 2 + kEpiWarps) {
     // ------------------------------------------------------------ scales into tensor memory
     if (lane == 0 && half == 0) {
+      const int part = warp - 2 - kEpiWarps;
       int slot = 0, set = 0, freed = 0;  // freed: the operand stage whose release frees the set
       uint32_t ph = 0, fph = 0;
       const int per = t0 < total ? (total - t0 - 1) / tstep + 1 : 0;
@@ -362,7 +365,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         tc_fence_after();
         const uint8_t* sf = smem + C::SF_OFF + slot * C::SF;
         const uint32_t sc = tmem_base + 256u + static_cast<uint32_t>(set * C::SF_COLS);
-        stage_scales<FMT, PAIR, BN>(sf, sf + C::SFA_BYTES, sc, sc + C::SFA_COLS);
+        if (part == 0) stage_scales<FMT, PAIR, BN, 0, 2>(sf, sf + C::SFA_BYTES, sc, sc + C::SFA_COLS);
+        else stage_scales<FMT, PAIR, BN, 1, 2>(sf, sf + C::SFA_BYTES, sc, sc + C::SFA_COLS);
         if constexpr (PAIR) umma_commit_pair(&sready[set]);
         else umma_commit(&sready[set]);
         if (++set == C::SETS) set = 0;
@@ -371,9 +375,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           ph ^= 1u;
         }
       }
-      if constexpr (PAIR) umma_commit_pair(drain + 1);
-      else umma_commit(drain + 1);
-      mbar_wait(drain + 1, 0, &g_status, kCodeDrain);
+      if constexpr (PAIR) umma_commit_pair(drain + 1 + part);
+      else umma_commit(drain + 1 + part);
+      mbar_wait(drain + 1 + part, 0, &g_status, kCodeDrain);
     }
     __syncwarp();
   } else {

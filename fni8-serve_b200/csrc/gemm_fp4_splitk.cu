@@ -7,9 +7,10 @@
 // are swapped (128 weight rows = MMA M, NT tokens = MMA N) and a cluster of S CTAs splits the
 // K range of a weight tile, S chosen so that the grid fills the GPU once; weights are loaded
 // before the wait for the quantiser. Here the S partial accumulators meet in shared memory:
-// CTA r owns 128 / S weight rows, every CTA stores the other ranks' rows of its accumulator
-// into their landing areas (distributed shared memory), and the owner adds the S parts in
-// rank order, so the result does not depend on timing and there is no workspace.
+// CTA r owns a share of the token columns, every CTA stores the columns of the others into
+// their landing areas (distributed shared memory, 16-byte pieces of four tokens, the weight row
+// innermost), and the owner adds the S parts in rank order, so the result does not depend on
+// timing and there is no workspace.
 #include <mutex>
 
 #include "fp4_common.cuh"
@@ -48,21 +49,8 @@ struct Cfg {
   static_assert(STAGE % 1024 == 0, "stages keep the 1024-byte alignment of the swizzle");
 };
 
-// weight rows that rank r of S owns: [r R, min(128, (r + 1) R))
-__host__ __device__ __forceinline__ int owned_rows(int S) { return (128 + S - 1) / S; }
-
-template <int FMT>
-__device__ __forceinline__ void put(const Epi& epi, float v, int m, int n, int N) {
-  if constexpr (FMT == FNI8_NVFP4) v = __fmul_rn(__fmul_rn(v, __ldg(epi.a_rs + m)), __ldg(epi.w_rs + n));
-  const int64_t at = static_cast<int64_t>(m) * N + n;
-  if (epi.bf16) {
-    if (epi.bias != nullptr) v = __fadd_rn(v, __bfloat162float(static_cast<const __nv_bfloat16*>(epi.bias)[n]));
-    static_cast<__nv_bfloat16*>(epi.out)[at] = __float2bfloat16_rn(v);
-  } else {
-    if (epi.bias != nullptr) v = __fadd_rn(v, __half2float(static_cast<const __half*>(epi.bias)[n]));
-    static_cast<__half*>(epi.out)[at] = __float2half_rn(v);
-  }
-}
+// token columns that rank r of S owns: [r share, (r + 1) share) of the first mcols
+__host__ __device__ __forceinline__ int column_share(int mcols, int S) { return ((mcols + S - 1) / S + 3) & ~3; }
 
 template <int FMT, int NT>
 __global__ void __launch_bounds__(kThreads, 2)
@@ -77,7 +65,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint64_t* tfull = empty + kMaxStages;
   uint64_t* drain = tfull + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
-  float* land = reinterpret_cast<float*>(smem + stages * C::STAGE + 256);  // [S][M][R]
+  float* s_ra = reinterpret_cast<float*>(smem + stages * C::STAGE + 256);                    // [NT]
+  uint4* land = reinterpret_cast<uint4*>(smem + stages * C::STAGE + 256 + NT * 4);  // [S][share / 4][128]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank()), S = static_cast<int>(cluster_nctarank());
@@ -107,6 +96,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 
   int okt = 0;
+  float rw = 1.0f, bias = 0.0f;  // of this epilogue thread's weight row
+  const int row = (warp & 3) * 32 + lane;  // epilogue warps 2-5 read the TMEM lanes of quarters 2, 3, 0, 1
+  const int n = tile * 128 + row;
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0) {
@@ -178,56 +170,95 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_wait(drain, 0, &g_status, kCodeDrain);
     }
   } else {
+    if (n < N) {
+      if constexpr (FMT == FNI8_NVFP4) rw = __ldg(epi.w_rs + n);
+      if (epi.bias != nullptr)
+        bias = epi.bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(epi.bias)[n])
+                        : __half2float(static_cast<const __half*>(epi.bias)[n]);
+    }
     pdl_wait();
+    if constexpr (FMT == FNI8_NVFP4) {
+      for (int m = threadIdx.x - 64; m < M; m += 128) s_ra[m] = __ldg(epi.a_rs + m);
+      named_bar_sync(1, 128);
+    }
     if (lane == 0) okt = mbar_wait(tfull, 0, &g_status, kCodeEpilogue) ? 1 : 0;
     okt = __shfl_sync(0xffffffffu, okt, 0);
     tc_fence_after();
   }
   __syncwarp();
-  pdl_wait();  // every thread may write out below
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 
-  const int row = (warp & 3) * 32 + lane;  // epilogue warps 2-5 read the TMEM lanes of quarters 2, 3, 0, 1
   const uint32_t taddr = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-  const int R = owned_rows(S);
-  if (warp >= 2 && okt) {
-    const int n = tile * 128 + row;
-    const int owner = row / R;
-    const uint32_t dst = mapa_shared(smem_u32(land), static_cast<uint32_t>(owner)) +
-                         static_cast<uint32_t>((rank * M * R + row - owner * R) * 4);
+  const int mcols = (M + 3) & ~3;
+  const int share = S > 1 ? column_share(mcols, S) : mcols;
+  if (S > 1) {
+    if (warp >= 2 && okt) {
+      const int g4 = share >> 2;
+      int owner = 0, first = 0;  // of the column at hand
+      uint32_t peer = mapa_shared(smem_u32(land), 0);
 #pragma unroll 1
-    for (int c0 = 0; c0 < M; c0 += 16) {
-      uint32_t r[16];
-      tmem_ld16(taddr + static_cast<uint32_t>(c0), r);
-      tmem_ld_wait();
+      for (int c0 = 0; c0 < mcols; c0 += 16) {
+        uint32_t r[16];
+        tmem_ld16(taddr + static_cast<uint32_t>(c0), r);
+        tmem_ld_wait();
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        if (c0 + j < M) {
-          if (S == 1) {
-            if (n < N) put<FMT>(epi, __uint_as_float(r[j]), c0 + j, n, N);
-          } else {
-            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst + static_cast<uint32_t>((c0 + j) * R * 4)), "r"(r[j])
-                         : "memory");
+        for (int j = 0; j < 16; j += 4) {
+          const int c = c0 + j;
+          if (c < mcols) {
+            if (c == first + share) {
+              first = c;
+              peer = mapa_shared(smem_u32(land), static_cast<uint32_t>(++owner));
+            }
+            if (owner != rank)
+              st_dsmem_v4(peer + static_cast<uint32_t>(((rank * g4 + ((c - first) >> 2)) * 128 + row) * 16),
+                          make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]));
           }
         }
       }
     }
-    tc_fence_before();
-  }
-  if (S > 1) {
     __syncwarp();
     cluster_sync_all();
-    pdl_launch_dependents();
-    const int rows = min(R, 128 - rank * R);
-    const int n0 = tile * 128 + rank * R;
-    for (int i = threadIdx.x; i < M * R; i += kThreads) {
-      const int m = i / R, r = i - m * R;
-      if (r < rows && n0 + r < N) {
-        float v = land[i];
-        for (int s = 1; s < S; ++s) v = __fadd_rn(v, land[s * M * R + i]);
-        put<FMT>(epi, v, m, n0 + r, N);
+  }
+  pdl_launch_dependents();
+  if (warp >= 2 && okt) {
+    const int own0 = rank * share, end = min(own0 + share, M), g4 = share >> 2;
+#pragma unroll 1
+    for (int c0 = own0; c0 < end; c0 += 16) {
+      uint32_t r[16];
+      tmem_ld16(taddr + static_cast<uint32_t>(c0), r);  // columns behind the accumulator are not used
+      tmem_ld_wait();
+      float v[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] = rank == 0 ? __uint_as_float(r[j]) : 0.0f;
+      for (int s = 0; s < S; ++s) {
+        if (s == 0 && rank == 0) continue;
+        const uint4* part = land + (s * g4 + ((c0 - own0) >> 2)) * 128 + row;
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          if (c0 + j < end) {
+            uint4 p = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+            if (s != rank) p = part[(j >> 2) * 128];
+            v[j] = __fadd_rn(v[j], __uint_as_float(p.x));
+            v[j + 1] = __fadd_rn(v[j + 1], __uint_as_float(p.y));
+            v[j + 2] = __fadd_rn(v[j + 2], __uint_as_float(p.z));
+            v[j + 3] = __fadd_rn(v[j + 3], __uint_as_float(p.w));
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int m = c0 + j;
+        if (m < end && n < N) {
+          float o = v[j];
+          if constexpr (FMT == FNI8_NVFP4) o = __fmul_rn(__fmul_rn(o, s_ra[m]), rw);
+          if (epi.bias != nullptr) o = __fadd_rn(o, bias);
+          const int64_t at = static_cast<int64_t>(m) * N + n;
+          if (epi.bf16) static_cast<__nv_bfloat16*>(epi.out)[at] = __float2bfloat16_rn(o);
+          else static_cast<__half*>(epi.out)[at] = __float2half_rn(o);
+        }
       }
     }
+    tc_fence_before();
   }
   __syncthreads();
   if (warp == 1) {
@@ -287,8 +318,8 @@ int launch_splitk(const Fp4Gemm& g, cudaStream_t st) {
   const int tiles = (int)((g.N + 127) / 128), kb = (int)((fp4::padded_k(g.K) + 255) / 256);
   // Ring: half an SM's shared memory (two CTAs per SM) up to 32 tokens, a whole SM's beyond.
   auto plan = [&](int S, int* stages) {
-    const int land = S > 1 ? S * (int)g.M * fp4s::owned_rows(S) * 4 : 0;
-    const int fixed = 1024 + 256 + land;
+    const int land = S > 1 ? S * fp4s::column_share(((int)g.M + 3) & ~3, S) * 128 * 4 : 0;
+    const int fixed = 1024 + 256 + NT * 4 + land;
     const int per = (kb + S - 1) / S;
     int n = ((NT <= 32 ? 113 : 225) * 1024 - fixed) / C::STAGE;
     n = n < fp4s::kMaxStages ? n : fp4s::kMaxStages;
