@@ -126,6 +126,94 @@ __device__ __forceinline__ void stage_mmas(uint32_t d, const void* sa, const voi
   }
 }
 
+// ---------------------------------------------------------------- quantisation of a chunk
+// Largest magnitude of eight values, as the bits of a float: an infinity or NaN wins.
+__device__ __forceinline__ uint32_t abs_max8(const float (&f)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7FFFFFFFu);
+  return m;
+}
+
+// 2^e of a float, e in [-127, 127]
+__device__ __forceinline__ float pow2f(int e) {
+  return __uint_as_float(e > -127 ? static_cast<uint32_t>(e + 127) << 23 : 0x00400000u);
+}
+
+// floor(log2(v)) of a positive float given by its bits
+__device__ __forceinline__ int floor_log2(uint32_t bits) {
+  const int e = static_cast<int>(bits >> 23);
+  return e > 0 ? e - 127 : -118 - __clz(bits);  // denormal: 2^-149 has one bit, 31 leading zeros
+}
+
+__device__ __forceinline__ uint32_t e2m1x8(const float (&f)[8]) {
+  uint32_t out;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(out)
+      : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]));
+  return out;
+}
+
+__device__ __forceinline__ uint32_t e4m3_bits(float v) {
+  uint16_t b;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b) : "f"(0.0f), "f"(v));
+  return b & 0xFF;
+}
+__device__ __forceinline__ float e4m3_value(uint32_t bits) {
+  uint32_t h2;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(static_cast<uint16_t>(bits)));
+  return __half2float(__ushort_as_half(static_cast<unsigned short>(h2 & 0xFFFF)));
+}
+
+constexpr uint32_t kInfBits = 0x7F800000u;
+
+// Codes and scale byte of a chunk of eight values whose block has the maximum `top` (the bits
+// of a float). nvfp4: row_exp is the row scale's exponent; f / (2^row_exp sf) is formed
+// without dividing by the row scale first, but for rows so small that 1 / (2^row_exp sf)
+// might not be a float.
+template <int FMT>
+__device__ __forceinline__ uint32_t chunk_codes(float (&f)[8], uint32_t top, int row_exp, uint32_t& scale) {
+  if constexpr (FMT == FNI8_MXFP4) {
+    int e = top == 0 ? -127 : floor_log2(top) - 2;
+    e = max(e, -127);
+    scale = top >= kInfBits ? 0xFFu : static_cast<uint32_t>(e + 127);
+    const float inv = pow2f(-e);  // e <= 125
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(f[i], inv);
+  } else {
+    const float unit = pow2f(-row_exp);
+    scale = top >= kInfBits ? 0x7Fu : e4m3_bits(__fdiv_rn(__fmul_rn(__uint_as_float(top), unit), 6.0f));
+    float d = top >= kInfBits ? 0.0f : e4m3_value(scale);  // 2^-9 .. 448, or 0
+    float inv = d > 0.0f ? __frcp_rn(d) : 0.0f;
+    if (row_exp < -100) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(f[i], unit);
+    } else {
+      d = __fmul_rn(d, pow2f(row_exp));  // exact, as is the next line
+      inv = __fmul_rn(inv, unit);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float q = __fmul_rn(f[i], inv);
+      f[i] = __fmaf_rn(-__fmaf_rn(q, d, -f[i]), inv, q);  // (in this order a zero keeps its sign)
+    }
+  }
+  return e2m1x8(f);
+}
+
+// Exponent of an nvfp4 row's scale from the bits of its largest magnitude: the least power of
+// two >= top / 2688, 2688 = 1.3125 * 2^11.
+__device__ __forceinline__ int row_exponent(uint32_t top) {
+  if (top == 0) return -126;
+  const int e = floor_log2(top);
+  return max(-126, (top >> 23) > 0 && (top & 0x7FFFFFu) > 0x280000u ? e - 10 : e - 11);
+}
+
 }  // namespace fp4
 }  // namespace fni8b
 

@@ -559,14 +559,25 @@ int check_gemm_fp4(const Fp4Gemm& g, int out_dtype) {
       (fp4::row_tiles(g.N) + 2) * fp4::k_tiles(g.format, g.K) * 4 >= lim)
     return fail(FNI8_ERR_UNSUPPORTED, "fp4 GEMM: sizes too large");
   if (g.M == 0) return FNI8_OK;
-  if (!g.a || !g.a_sf || !g.w || !g.w_sf || !g.out) return fail(FNI8_ERR_INVALID, "null GEMM operand");
-  if (g.format == FNI8_NVFP4 && (!g.a_rs || !g.w_rs)) return fail(FNI8_ERR_INVALID, "nvfp4 GEMM: null row scale");
-  if ((reinterpret_cast<uintptr_t>(g.a) | reinterpret_cast<uintptr_t>(g.w) | reinterpret_cast<uintptr_t>(g.a_sf) |
-       reinterpret_cast<uintptr_t>(g.w_sf)) & 15u)
+  if (!g.w || !g.w_sf || !g.out) return fail(FNI8_ERR_INVALID, "null GEMM operand");
+  if (g.format == FNI8_NVFP4 && !g.w_rs) return fail(FNI8_ERR_INVALID, "nvfp4 GEMM: null row scale");
+  if ((reinterpret_cast<uintptr_t>(g.w) | reinterpret_cast<uintptr_t>(g.w_sf)) & 15u)
     return fail(FNI8_ERR_ALIGN, "fp4 GEMM: codes and scales must be 16-byte aligned");
   if ((reinterpret_cast<uintptr_t>(g.out) | reinterpret_cast<uintptr_t>(g.bias)) & 1u)
     return fail(FNI8_ERR_ALIGN, "fp4 GEMM: out and bias must be 2-byte aligned");
   return FNI8_OK;
+}
+
+// Scratch of fni8_linear_fp4: scale tiles, codes, row scales.
+struct Fp4Scratch {
+  size_t q, rs, total;
+};
+Fp4Scratch fp4_scratch(int format, int64_t M, int64_t K) {
+  Fp4Scratch s;
+  s.q = fni8_fp4_scale_bytes(format, M, K);
+  s.rs = s.q + static_cast<size_t>(M) * (fp4::padded_k(K) / 2);
+  s.total = s.rs + static_cast<size_t>(M) * 4;
+  return s;
 }
 
 }  // namespace
@@ -580,18 +591,39 @@ extern "C" int fni8_gemm_fp4(const uint8_t* a, const uint8_t* a_sf, const float*
   const Fp4Gemm g{a, a_sf, a_row_scale, w, w_sf, w_row_scale, bias, out, out_dtype == FNI8_BF16, format, M, N, K};
   if (int s = check_gemm_fp4(g, out_dtype)) return s;
   if (M == 0) return FNI8_OK;
+  if (!a || !a_sf) return fail(FNI8_ERR_INVALID, "null GEMM operand");
+  if (format == FNI8_NVFP4 && !a_row_scale) return fail(FNI8_ERR_INVALID, "nvfp4 GEMM: null row scale");
+  if ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(a_sf)) & 15u)
+    return fail(FNI8_ERR_ALIGN, "fp4 GEMM: codes and scales must be 16-byte aligned");
   return run_gemm(g, static_cast<cudaStream_t>(stream));
 }
 
+extern "C" size_t fni8_linear_fp4_scratch_bytes(int format, int64_t M, int64_t N, int64_t K) {
+  if ((format != FNI8_MXFP4 && format != FNI8_NVFP4) || M <= 0 || N <= 0 || K <= 0) return 0;
+  return fp4_fused_supported(format, M, N, K) ? 0 : fp4_scratch(format, M, K).total;
+}
+
 extern "C" int fni8_linear_fp4(const void* x, int dtype, const uint8_t* w, const uint8_t* w_sf, const float* w_row_scale,
-                               const void* bias, void* out, int format, int64_t M, int64_t N, int64_t K,
-                               uint8_t* q_scratch, uint8_t* sf_scratch, float* rs_scratch, void* stream) {
-  if (int s = fp4_check_rows(x, dtype, format, M, K, q_scratch, sf_scratch, rs_scratch)) return s;
-  const Fp4Gemm g{q_scratch, sf_scratch, rs_scratch, w, w_sf, w_row_scale, bias, out, dtype == FNI8_BF16, format, M, N,
-                  K};
+                               const void* bias, void* out, int format, int64_t M, int64_t N, int64_t K, void* scratch,
+                               size_t scratch_bytes, void* stream) {
+  Fp4Gemm g{nullptr, nullptr, nullptr, w, w_sf, w_row_scale, bias, out, dtype == FNI8_BF16, format, M, N, K};
   if (int s = check_gemm_fp4(g, dtype)) return s;
   if (M == 0) return FNI8_OK;
+  if (!x) return fail(FNI8_ERR_INVALID, "null linear input");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (int s = fp4_quantize(x, dtype, format, M, K, false, q_scratch, sf_scratch, rs_scratch, st)) return s;
+  const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
+  if (aligned && fp4_fused_supported(format, M, N, K)) return fp4_fused(g, x, st);
+  const Fp4Scratch sc = fp4_scratch(format, M, K);
+  if (!scratch || scratch_bytes < sc.total) {
+    if (!aligned && fp4_fused_supported(format, M, N, K))
+      return fail(FNI8_ERR_ALIGN, "fp4 linear: x must be 16-byte aligned to run without scratch");
+    return fail(FNI8_ERR_WORKSPACE, "fp4 linear needs %zu scratch bytes (got %zu)", sc.total, scratch_bytes);
+  }
+  uint8_t* b = static_cast<uint8_t*>(scratch);
+  g.a_sf = b;
+  g.a = b + sc.q;
+  g.a_rs = reinterpret_cast<float*>(b + sc.rs);
+  if (int s = fp4_check_rows(x, dtype, format, M, K, b + sc.q, b, reinterpret_cast<float*>(b + sc.rs))) return s;
+  if (int s = fp4_quantize(x, dtype, format, M, K, false, b + sc.q, b, reinterpret_cast<float*>(b + sc.rs), st)) return s;
   return run_gemm(g, st);
 }

@@ -101,6 +101,9 @@ int fp4_quantize(const void* x, int dtype, int format, int64_t M, int64_t K, boo
                  float* row_scale, cudaStream_t st);
 // The swap-AB split-K kernel for M <= 128 (gemm_fp4_splitk.cu).
 int fp4_splitk(const Fp4Gemm& g, cudaStream_t st);
+// Its form that quantises the 16-bit rows x itself (16-byte aligned; a, a_sf and a_rs unused).
+bool fp4_fused_supported(int format, int64_t M, int64_t N, int64_t K);
+int fp4_fused(const Fp4Gemm& g, const void* x, cudaStream_t st);
 int fp4_status_read_and_clear(int* code);
 int fp4s_status_read_and_clear(int* code);
 

@@ -47,7 +47,8 @@ SIGNATURES: dict[str, tuple] = {
     "fni8_quantize_rows_fp4": (_i, [_p, _i, _i, _i64, _i64, _p, _p, _p, _p]),
     "fni8_dequantize_rows_fp4": (_i, [_p, _p, _p, _i, _i64, _i64, _p, _i, _p]),
     "fni8_gemm_fp4": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i64, _i64, _i64, _p]),
-    "fni8_linear_fp4": (_i, [_p, _i, _p, _p, _p, _p, _p, _i, _i64, _i64, _i64, _p, _p, _p, _p]),
+    "fni8_linear_fp4_scratch_bytes": (_sz, [_i, _i64, _i64, _i64]),
+    "fni8_linear_fp4": (_i, [_p, _i, _p, _p, _p, _p, _p, _i, _i64, _i64, _i64, _p, _sz, _p]),
     "fni8_gemm_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "fni8_workspace_init": (_i, [_p, _sz, _p]),
     "fni8_gemm_w8a8": (_i, [_p, _p, _p, _p, _p, _p, _p, _i, _i64, _i64, _i64, _p, _sz, _p]),

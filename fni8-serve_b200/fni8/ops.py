@@ -491,14 +491,13 @@ def _linear_fp4(x: torch.Tensor, qt: QTensor, bias: torch.Tensor | None) -> torc
     M = x2.shape[0]
     b = _fp4_bias(bias, N, x.dtype, dev, "linear")
     out = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev)
-    # one scratch: scale tiles, codes, row scales (each part a multiple of 16 bytes)
-    sf_bytes = (M + 127) // 128 * ((K + 4 * g - 1) // (4 * g)) * 512
-    q_bytes = M * ((K + 31) // 32 * 16)
-    scratch = torch.empty(sf_bytes + q_bytes + 4 * M, dtype=torch.uint8, device=dev)
-    sf = scratch.data_ptr()
+    sb = nat.lib().fni8_linear_fp4_scratch_bytes(fmt, M, N, K)  # 0: one kernel that quantises x itself
+    if sb == 0 and x2.data_ptr() & 15:
+        x2 = x2.clone()
+    scratch = torch.empty(sb, dtype=torch.uint8, device=dev) if sb else None
     with torch.cuda.device(dev):
         nat.call("fni8_linear_fp4", _vp(x2), dt, _vp(qt.data), _vp(qt.scale), _vp(qt.row_scale), _vp(b), _vp(out), fmt,
-                 M, N, K, sf + sf_bytes, sf, sf + sf_bytes + q_bytes, _stream(dev))
+                 M, N, K, _vp(scratch), sb, _stream(dev))
     return out
 
 

@@ -272,11 +272,15 @@ FNI8_API int fni8_gemm_fp4(const uint8_t* a, const uint8_t* a_sf, const float* a
                            const uint8_t* w_sf, const float* w_row_scale, const void* bias, void* out, int out_dtype,
                            int format, int64_t M, int64_t N, int64_t K, void* stream);
 /* fni8.linear(x, qt, bias=) for FNI8_MXFP4 / FNI8_NVFP4 weights: x[M, K] quantised to the
- * weight's format into q_scratch [M, Kp / 2], sf_scratch (fni8_fp4_scale_bytes) and, for
- * FNI8_NVFP4, rs_scratch [M], then fni8_gemm_fp4 into out[M, N] (dtype of x). */
+ * weight's format, then fni8_gemm_fp4 into out[M, N] (dtype of x); the result is that of the
+ * two calls, bit for bit. Up to 16 rows of 16-byte aligned x (K a multiple of 8) run in one
+ * kernel that quantises x itself, where a slice of the rows fits beside the weights; then
+ * fni8_linear_fp4_scratch_bytes is 0 and scratch may be NULL. Otherwise scratch holds the
+ * quantised rows (16-byte aligned). */
+FNI8_API size_t fni8_linear_fp4_scratch_bytes(int format, int64_t M, int64_t N, int64_t K);
 FNI8_API int fni8_linear_fp4(const void* x, int dtype, const uint8_t* w, const uint8_t* w_sf, const float* w_row_scale,
-                             const void* bias, void* out, int format, int64_t M, int64_t N, int64_t K,
-                             uint8_t* q_scratch, uint8_t* sf_scratch, float* rs_scratch, void* stream);
+                             const void* bias, void* out, int format, int64_t M, int64_t N, int64_t K, void* scratch,
+                             size_t scratch_bytes, void* stream);
 
 /* ------------------------------------------------------------------ MoE */
 /* Router scores -> top-k (SparseMoE.forward routing, fni8serve/models/moe.py:65-95):

@@ -106,11 +106,19 @@ def test_c_abi_refusals():
     assert gemm(out=p + 1) == n.ERR_ALIGN and gemm(bias=p + 1) == n.ERR_ALIGN
     assert gemm(M=0, a=None) == n.OK
 
-    def linear(x=p, dt=n.BF16, fmt=n.NVFP4, M=4, N=8, K=64, q=p, sf=p, rs=p, w=p):
-        return L.fni8_linear_fp4(x, dt, w, p, p, None, p, fmt, M, N, K, q, sf, rs, None)
+    def linear(x=p, dt=n.BF16, fmt=n.NVFP4, M=40, N=8, K=64, w=p, scratch=p, sb=1 << 20):
+        return L.fni8_linear_fp4(x, dt, w, p, p, None, p, fmt, M, N, K, scratch, sb, None)
 
-    assert linear(x=None) == n.ERR_INVALID and linear(q=None) == n.ERR_INVALID and linear(rs=None) == n.ERR_INVALID
-    assert linear(dt=n.I32) == n.ERR_INVALID and linear(w=None) == n.ERR_INVALID and linear(N=-3) == n.ERR_INVALID
+    assert linear(x=None) == n.ERR_INVALID and linear(w=None) == n.ERR_INVALID and linear(N=-3) == n.ERR_INVALID
+    assert linear(dt=n.I32) == n.ERR_INVALID and linear(fmt=3) == n.ERR_INVALID
+    need = L.fni8_linear_fp4_scratch_bytes(n.NVFP4, 40, 8, 64)
+    assert need == 512 + 40 * 32 + 40 * 4
+    assert linear(scratch=None) == n.ERR_WORKSPACE and linear(sb=need - 1) == n.ERR_WORKSPACE
+    assert linear(scratch=bad) == n.ERR_ALIGN and linear(x=p + 1) == n.ERR_ALIGN
+    assert L.fni8_linear_fp4_scratch_bytes(n.NVFP4, 16, 8, 64) == 0  # one kernel
+    assert linear(M=16, x=bad, scratch=None, sb=0) == n.ERR_ALIGN
+    assert L.fni8_linear_fp4_scratch_bytes(n.NVFP4, 16, 8, 63) > 0 and linear(M=16, K=63, sb=0) == n.ERR_WORKSPACE
+    assert L.fni8_linear_fp4_scratch_bytes(9, 16, 8, 64) == 0 and L.fni8_linear_fp4_scratch_bytes(0, 0, 8, 64) == 0
     assert linear(M=0, x=None) == n.OK
     assert L.fni8_fp4_scale_bytes(n.MXFP4, 130, 129) == 2 * 2 * 512
     assert L.fni8_fp4_scale_bytes(n.NVFP4, 1, 64) == 512

@@ -308,3 +308,24 @@ def test_refusals_on_the_gpu():
         fni8.dequantize_fp4(w, torch.int8)
     with pytest.raises(RuntimeError):
         fni8.linear(x, w.to("cpu"))
+
+
+@pytest.mark.parametrize("scheme", SCHEMES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N,K", [(1, 128, 8), (1, 129, 256), (3, 6144, 4096), (16, 96, 1000), (7, 4096, 12288),
+                                   (16, 20000, 520), (5, 40000, 2048), (9, 300, 8200), (2, 130, 16384), (17, 200, 4096)])
+def test_linear_in_one_kernel(scheme, dtype, M, N, K):
+    """Up to 16 rows linear quantises them in the GEMM: the result of the two calls bit for bit, also with rows of
+    very different size, an all-zero row, and from misaligned rows (which take the two kernels)."""
+    import fni8
+
+    x = rows(M, K, dtype, M + K).to(DEV)
+    w, _ = random_qt(N, K, scheme, N, False)
+    bias = torch.randn(N, generator=gen(3)).to(dtype).to(DEV)
+    want = fni8.linear_fp4(fni8.quantize_fp4(x, scheme), w, bias=bias, out_dtype=dtype)
+    for _ in range(2):
+        assert torch.equal(fni8.linear(x, w, bias=bias), want)
+    flat = torch.empty(M * K + 1, dtype=dtype, device=DEV)
+    flat[1:] = x.reshape(-1)
+    assert torch.equal(fni8.linear(flat[1:].view(M, K), w, bias=bias), want)
+    assert fni8.device_status() == 0
