@@ -5,41 +5,47 @@
 // produce exactly their roundings:
 //   * dividing by a power of two is exact (a float holds every quotient that matters: a
 //     denormal one rounds to code 0 either way);
-//   * max / 6 is an IEEE division. max has at most 11 significant bits, so max / 6 either
-//     is a midpoint of e4m3 (then the quotient is exact) or is at least 2^-17 of itself
-//     away from one, further than the division's rounding;
-//   * x / sf is v * (1 / sf), corrected once by its fused remainder (Markstein's step). With
-//     11 bits in x and 4 in sf the same argument holds for the midpoints of e2m1.
+//   * max / 6 and x / sf are products with the reciprocal, corrected once by their fused
+//     remainders (BlockScale), which leaves the quotient's own rounding, or its neighbour in
+//     rare cases. max has at most 11 significant bits, so max / 6 either is a midpoint of e4m3
+//     (then the quotient is a float and exact) or is at least 2^-17 of itself away from one,
+//     further than any rounding here. With 11 bits in x and 4 in sf the same holds for x / sf
+//     and the midpoints of e2m1.
 // Nothing of a row depends on another row.
 //
-// A row belongs to 32, 128, 256 or 512 threads, eight values (one 16-byte load; half or a quarter of
-// a block) to a thread and step. An nvfp4 row stays in registers while its maximum is found,
-// so it is read once, up to 16384 values.
-// Bound: HBM, 2 bytes read and 1/2 + 1/g written per value.
+// A row belongs to 32, 128, 256 or 512 threads, sixteen values to a thread and step (an nvfp4
+// block, half of an mxfp4 one: with eight, the scale's arithmetic was done twice as often and
+// an nvfp4 8192 x 4096 took 25 us, 80 % of the issue slots). An nvfp4 row stays in registers
+// while its maximum is found, so it is read once, up to 16384 values.
+// Bound: HBM, 2 bytes read and 1/2 + 1/g written per value; the issue rate comes next.
 #include "fp4_common.cuh"
 #include "gemm_internal.h"
 
 namespace fni8b {
 namespace fp4 {
 
-// Eight values of a row from k on, zeros behind K. VW values to a load (the largest power of
-// two that the rows' alignment allows).
+struct Raw16 {  // sixteen 16-bit values
+  uint4 lo, hi;
+};
+
+// The values of a row from k on, zeros behind K. VW values to a load (the largest power of two
+// that the rows' alignment allows).
 template <typename T, int VW>
-__device__ __forceinline__ uint4 load8(const T* __restrict__ row, int64_t k, int64_t K) {
-  alignas(16) T v[8];
-  if (k + 8 <= K) {
+__device__ __forceinline__ Raw16 load16(const T* __restrict__ row, int64_t k, int64_t K) {
+  alignas(16) T v[16];
+  if (k + 16 <= K) {
 #pragma unroll
-    for (int i = 0; i < 8; i += VW) {
-      if constexpr (VW == 8) *reinterpret_cast<uint4*>(v) = __ldg(reinterpret_cast<const uint4*>(row + k));
+    for (int i = 0; i < 16; i += VW) {
+      if constexpr (VW == 8) *reinterpret_cast<uint4*>(v + i) = __ldg(reinterpret_cast<const uint4*>(row + k + i));
       else if constexpr (VW == 4) *reinterpret_cast<uint2*>(v + i) = __ldg(reinterpret_cast<const uint2*>(row + k + i));
       else if constexpr (VW == 2) *reinterpret_cast<uint32_t*>(v + i) = __ldg(reinterpret_cast<const uint32_t*>(row + k + i));
       else v[i] = row[k + i];
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = k + i < K ? row[k + i] : from_f32<T>(0.0f);
+    for (int i = 0; i < 16; ++i) v[i] = k + i < K ? row[k + i] : from_f32<T>(0.0f);
   }
-  return *reinterpret_cast<const uint4*>(v);
+  return Raw16{*reinterpret_cast<const uint4*>(v), *reinterpret_cast<const uint4*>(v + 8)};
 }
 
 template <typename T>
@@ -49,11 +55,14 @@ __device__ __forceinline__ void unpack8(const uint4& u, float (&f)[8]) {
   for (int i = 0; i < 8; ++i) f[i] = to_f32<T>(v[i]);
 }
 
-// Largest magnitude of eight values as the bits of a float (an infinity or NaN wins): the
-// order of the 16-bit patterns without their signs.
+// Largest magnitude as the bits of a float (an infinity or NaN wins): the order of the 16-bit
+// patterns without their signs.
 template <typename T>
-__device__ __forceinline__ uint32_t raw_max8(const uint4& u) {
-  const uint32_t m = __vmaxu2(__vmaxu2(u.x & 0x7FFF7FFFu, u.y & 0x7FFF7FFFu), __vmaxu2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu));
+__device__ __forceinline__ uint32_t raw_max(const Raw16& r) {
+  auto four = [](const uint4& u) {
+    return __vmaxu2(__vmaxu2(u.x & 0x7FFF7FFFu, u.y & 0x7FFF7FFFu), __vmaxu2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu));
+  };
+  const uint32_t m = __vmaxu2(four(r.lo), four(r.hi));
   const unsigned short top = static_cast<unsigned short>(max(m & 0xFFFFu, m >> 16));
   return __float_as_uint(to_f32<T>(*reinterpret_cast<const T*>(&top)));
 }
@@ -66,46 +75,45 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP) quant_rows(const T*
                                                                         uint8_t* __restrict__ sf,
                                                                         float* __restrict__ row_scale) {
   constexpr int kThreads = GROUP < 128 ? 128 : GROUP;
-  constexpr int kLanes = Fmt<FMT>::kBlock / 8;  // threads that share a block
-  constexpr int kWordLanes = 4 * kLanes;        // threads that share a cell of four scales
+  constexpr int kLanes = Fmt<FMT>::kBlock / 16;  // threads that share a block
+  constexpr int kWordLanes = 4 * kLanes;         // threads that share a cell of four scales
   __shared__ uint32_t red[kThreads / 32];
   pdl_launch_dependents();
   pdl_wait();
   const int g = threadIdx.x / GROUP, t = threadIdx.x % GROUP, lane = threadIdx.x & 31;
   const int64_t tiles = k_tiles(FMT, K);
   const int chunks = static_cast<int>(tiles * kWordLanes);  // with the last cell's zero scales
-  const int code_chunks = static_cast<int>(padded_k(K) / 8);
+  const int code_chunks = static_cast<int>(padded_k(K) / 16);
   const int64_t stride = static_cast<int64_t>(gridDim.x) * (kThreads / GROUP);
+  const Raw16 zero{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
   // a CTA's groups take the same number of rounds (they meet at barriers)
   for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kThreads / GROUP); row0 < pad_rows; row0 += stride) {
     const int64_t row = row0 + g;
     const bool real = row < M;
     const T* xr = x + row * K;
-    uint32_t* qr = reinterpret_cast<uint32_t*>(q + row * (padded_k(K) / 2));
+    uint2* qr = reinterpret_cast<uint2*>(q + row * (padded_k(K) / 2));
     uint8_t* sr = sf + (row >> 7) * tiles * 512 + row_byte(static_cast<int>(row & 127));
     int row_exp = 0;
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    uint4 kept[KEEP > 0 ? KEEP : 1];
+    Raw16 kept[KEEP > 0 ? KEEP : 1];
     if constexpr (KEEP > 0) {
 #pragma unroll
-      for (int i = 0; i < KEEP; ++i) kept[i] = real ? load8<T, VW>(xr, static_cast<int64_t>(t + i * GROUP) * 8, K) : zero;
+      for (int i = 0; i < KEEP; ++i)
+        kept[i] = real ? load16<T, VW>(xr, static_cast<int64_t>(t + i * GROUP) * 16, K) : zero;
     }
     if constexpr (FMT == FNI8_NVFP4) {
       // the row's largest finite block: a block with an infinity or NaN stands for itself alone
       uint32_t top = 0;
-      auto enter = [&](const uint4& u) {
-        uint32_t m = raw_max8<T>(u);
-#pragma unroll
-        for (int o = 1; o < kLanes; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      auto enter = [&](const Raw16& r) {
+        const uint32_t m = raw_max<T>(r);
         if (m < kInfBits) top = max(top, m);
       };
       if constexpr (KEEP > 0) {
 #pragma unroll
         for (int i = 0; i < KEEP; ++i) enter(kept[i]);
       } else {
-#pragma unroll 4
+#pragma unroll 2
         for (int c0 = 0; c0 < chunks; c0 += GROUP)
-          enter(real ? load8<T, VW>(xr, static_cast<int64_t>(c0 + t) * 8, K) : zero);
+          enter(real ? load16<T, VW>(xr, static_cast<int64_t>(c0 + t) * 16, K) : zero);
       }
       top = __reduce_max_sync(0xffffffffu, top);
       if constexpr (GROUP > 32) {
@@ -118,18 +126,20 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP) quant_rows(const T*
       row_exp = row_exponent(top);
       if (real && t == 0) row_scale[row] = pow2f(row_exp);
     }
-    auto emit = [&](int c, const uint4& u) {
-      uint32_t top = raw_max8<T>(u), scale;
+    auto emit = [&](int c, const Raw16& r) {
+      uint32_t top = raw_max<T>(r);
+      if constexpr (kLanes == 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      const BlockScale<FMT> scale(top, row_exp);
       float f[8];
-      unpack8<T>(u, f);
-#pragma unroll
-      for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const uint32_t codes = chunk_codes<FMT>(f, top, row_exp, scale);
+      unpack8<T>(r.lo, f);
+      const uint32_t lo = scale.codes(f);
+      unpack8<T>(r.hi, f);
+      const uint32_t hi = scale.codes(f);
       // the cell's four scale bytes, from its blocks' lanes
-      uint32_t word = real ? scale << (8 * ((lane / kLanes) & 3)) : 0u;
+      uint32_t word = real ? scale.byte << (8 * ((lane / kLanes) & 3)) : 0u;
 #pragma unroll
       for (int o = kLanes; o < kWordLanes; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
-      if (real && c < code_chunks) qr[c] = codes;
+      if (real && c < code_chunks) qr[c] = make_uint2(lo, hi);
       if (row < pad_rows && c < chunks && (lane & (kWordLanes - 1)) == 0)
         *reinterpret_cast<uint32_t*>(sr + static_cast<int64_t>(c / kWordLanes) * 512) = word;
     };
@@ -138,9 +148,9 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP) quant_rows(const T*
       for (int i = 0; i < KEEP; ++i)
         if (i * GROUP < chunks) emit(t + i * GROUP, kept[i]);
     } else {
-#pragma unroll 4
+#pragma unroll 2
       for (int c0 = 0; c0 < chunks; c0 += GROUP)
-        emit(c0 + t, real ? load8<T, VW>(xr, static_cast<int64_t>(c0 + t) * 8, K) : zero);
+        emit(c0 + t, real ? load16<T, VW>(xr, static_cast<int64_t>(c0 + t) * 16, K) : zero);
     }
   }
 }
@@ -223,26 +233,25 @@ int check_fp4_rows(int format, int64_t M, int64_t K, const char* what) {
 template <typename T, int FMT, int VW>
 void launch_quant(const T* x, int64_t M, int64_t K, int64_t pad_rows, uint8_t* q, uint8_t* sf, float* rs,
                   cudaStream_t st) {
-  const int64_t chunks = fp4::k_tiles(FMT, K) * 4 * (fp4::Fmt<FMT>::kBlock / 8);
-  const int64_t blocks = chunks <= 128 ? (pad_rows + 3) / 4 : pad_rows;
+  const int64_t chunks = fp4::k_tiles(FMT, K) * 4 * (fp4::Fmt<FMT>::kBlock / 16);
+  const int64_t blocks = chunks <= 64 ? (pad_rows + 3) / 4 : pad_rows;
   const dim3 grid((unsigned)(blocks < 148 * 64 ? blocks : 148 * 64));
 #define FNI8_QUANT_FP4(G, KEEP)                                                                                     \
   launch_pdl(fp4::quant_rows<T, FMT, VW, G, KEEP>, grid, dim3(G < 128 ? 128 : G), 0, st, x, M, K, pad_rows, q, sf, rs)
-  // few long rows: more threads to each (1 x 12288 nvfp4 4.2 us with 512, 7.7 with 128)
+  // few long rows: more threads to each (1 x 12288 nvfp4 2.9 us with 512, 7.7 with 128)
   const bool few = M < 4 * 148;
   if constexpr (FMT == FNI8_MXFP4) {  // no row maximum: nothing to keep
-    if (chunks <= 32) FNI8_QUANT_FP4(32, 1);
-    else if (chunks <= 128) FNI8_QUANT_FP4(32, 0);
-    else if (few && chunks > 512) FNI8_QUANT_FP4(512, 0);
+    if (chunks <= 64) FNI8_QUANT_FP4(32, 0);
+    else if (few && chunks > 256) FNI8_QUANT_FP4(512, 0);
     else FNI8_QUANT_FP4(128, 0);
   } else {
     if (chunks <= 32) FNI8_QUANT_FP4(32, 1);
-    else if (chunks <= 128) FNI8_QUANT_FP4(32, 4);
+    else if (chunks <= 64) FNI8_QUANT_FP4(32, 2);
+    else if (chunks <= 128) FNI8_QUANT_FP4(128, 1);
     else if (chunks <= 256) FNI8_QUANT_FP4(128, 2);
-    else if (chunks <= 512) FNI8_QUANT_FP4(128, 4);
-    else if (few && chunks <= 2048) FNI8_QUANT_FP4(512, 4);
+    else if (few && chunks <= 1024) FNI8_QUANT_FP4(512, 2);
+    else if (chunks <= 512) FNI8_QUANT_FP4(256, 2);
     else if (chunks <= 1024) FNI8_QUANT_FP4(256, 4);
-    else if (chunks <= 2048) FNI8_QUANT_FP4(256, 8);
     else FNI8_QUANT_FP4(512, 0);
   }
 #undef FNI8_QUANT_FP4

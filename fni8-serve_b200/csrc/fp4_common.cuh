@@ -172,39 +172,60 @@ __device__ __forceinline__ float e4m3_value(uint32_t bits) {
 
 constexpr uint32_t kInfBits = 0x7F800000u;
 
-// Codes and scale byte of a chunk of eight values whose block has the maximum `top` (the bits
-// of a float). nvfp4: row_exp is the row scale's exponent; f / (2^row_exp sf) is formed
-// without dividing by the row scale first, but for rows so small that 1 / (2^row_exp sf)
-// might not be a float.
+// The scale of a block with the maximum `top` (the bits of a float; an infinity or NaN makes it
+// NaN), and what eight values of it need for their codes. nvfp4: row_exp is the exponent of
+// the row scale; f / (2^row_exp sf) is formed without dividing by the row scale first, but
+// for rows so small that 1 / (2^row_exp sf) might not be a float.
 template <int FMT>
-__device__ __forceinline__ uint32_t chunk_codes(float (&f)[8], uint32_t top, int row_exp, uint32_t& scale) {
-  if constexpr (FMT == FNI8_MXFP4) {
-    int e = top == 0 ? -127 : floor_log2(top) - 2;
-    e = max(e, -127);
-    scale = top >= kInfBits ? 0xFFu : static_cast<uint32_t>(e + 127);
-    const float inv = pow2f(-e);  // e <= 125
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(f[i], inv);
-  } else {
-    const float unit = pow2f(-row_exp);
-    scale = top >= kInfBits ? 0x7Fu : e4m3_bits(__fdiv_rn(__fmul_rn(__uint_as_float(top), unit), 6.0f));
-    float d = top >= kInfBits ? 0.0f : e4m3_value(scale);  // 2^-9 .. 448, or 0
-    float inv = d > 0.0f ? __frcp_rn(d) : 0.0f;
-    if (row_exp < -100) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(f[i], unit);
+struct BlockScale {
+  uint32_t byte;
+  float inv, d, pre;
+
+  __device__ __forceinline__ BlockScale(uint32_t top, int row_exp) {
+    if constexpr (FMT == FNI8_MXFP4) {
+      const int e = max(top == 0 ? -127 : floor_log2(top) - 2, -127);
+      byte = top >= kInfBits ? 0xFFu : static_cast<uint32_t>(e + 127);
+      inv = pow2f(-e);  // e <= 125
     } else {
-      d = __fmul_rn(d, pow2f(row_exp));  // exact, as is the next line
-      inv = __fmul_rn(inv, unit);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float q = __fmul_rn(f[i], inv);
-      f[i] = __fmaf_rn(-__fmaf_rn(q, d, -f[i]), inv, q);  // (in this order a zero keeps its sign)
+      // max / 6, corrected like the quotients below
+      const float t = __fmul_rn(__uint_as_float(top), pow2f(-row_exp)), sixth = 1.0f / 6.0f;
+      const float q = __fmul_rn(t, sixth);
+      byte = top >= kInfBits ? 0x7Fu : e4m3_bits(__fmaf_rn(__fmaf_rn(-q, 6.0f, t), sixth, q));
+      d = top >= kInfBits ? 0.0f : e4m3_value(byte);  // 2^-9 .. 448, or 0
+      float r;
+      asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(d));
+      inv = d > 0.0f ? r : 0.0f;
+      pre = 1.0f;
+      if (row_exp < -100) {
+        pre = pow2f(-row_exp);
+      } else {
+        d = __fmul_rn(d, pow2f(row_exp));  // exact, as is the next line
+        inv = __fmul_rn(inv, pow2f(-row_exp));
+      }
     }
   }
-  return e2m1x8(f);
-}
+
+  // Eight values' codes. nvfp4: q = f inv is the quotient but for a few units in the last
+  // place; its fused remainder f - q d is exact and corrects it to the quotient's rounding
+  // (Markstein's step, as in div_by_ge1).
+  __device__ __forceinline__ uint32_t codes(float (&f)[8]) const {
+    if constexpr (FMT == FNI8_MXFP4) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(f[i], inv);
+    } else {
+      if (pre != 1.0f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(f[i], pre);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float q = __fmul_rn(f[i], inv);
+        f[i] = __fmaf_rn(-__fmaf_rn(q, d, -f[i]), inv, q);  // (in this order a zero keeps its sign)
+      }
+    }
+    return e2m1x8(f);
+  }
+};
 
 // Exponent of an nvfp4 row's scale from the bits of its largest magnitude: the least power of
 // two >= top / 2688, 2688 = 1.3125 * 2^11.

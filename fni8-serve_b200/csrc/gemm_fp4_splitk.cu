@@ -151,12 +151,12 @@ __device__ __forceinline__ void quantise_slice(const Epi& epi, int M, int kbeg, 
     unpack(b, f);
     const uint32_t top = block_top(f);
     const int row_exp = FMT == FNI8_NVFP4 ? static_cast<int>(__float_as_uint(s_ra[m]) >> 23) - 127 : 0;
-    uint32_t scale;
-    const uint32_t codes = chunk_codes<FMT>(f, top, row_exp, scale);
+    const BlockScale<FMT> scale(top, row_exp);
+    const uint32_t codes = scale.codes(f);
     uint8_t* st = xs + (c >> 5) * C::X_STAGE;
     *reinterpret_cast<uint32_t*>(st + m * 128 + ((((c & 31) >> 2) ^ (m & 7)) << 4) + (c & 3) * 4) = codes;
     const int s = (c & 31) / kLanes;
-    if (lane % kLanes == 0) st[C::X_BYTES + (s >> 2) * 512 + m * 16 + (s & 3)] = static_cast<uint8_t>(scale);
+    if (lane % kLanes == 0) st[C::X_BYTES + (s >> 2) * 512 + m * 16 + (s & 3)] = static_cast<uint8_t>(scale.byte);
   }
   fence_proxy_async_smem();  // read by the tensor core
 }
