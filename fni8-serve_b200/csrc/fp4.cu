@@ -166,7 +166,8 @@ __global__ void __launch_bounds__(256) dequant_rows(const uint8_t* __restrict__ 
   pdl_wait();
   const int per_row = static_cast<int>((K + 7) / 8);
   const int64_t tiles = k_tiles(FMT, K), row_bytes = padded_k(K) / 2;
-  for (int64_t row = blockIdx.x; row < M; row += gridDim.x) {
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; row < M;
+       row += static_cast<int64_t>(gridDim.x) * blockDim.y) {
     const float rs = FMT == FNI8_NVFP4 ? __ldg(row_scale + row) : 1.0f;
     const uint8_t* sr = sf + (row >> 7) * tiles * 512 + row_byte(static_cast<int>(row & 127));
     const uint32_t* qr = reinterpret_cast<const uint32_t*>(q + row * row_bytes);
@@ -327,10 +328,15 @@ extern "C" int fni8_dequantize_rows_fp4(const uint8_t* q, const uint8_t* sf, con
   if (reinterpret_cast<uintptr_t>(out) % esz != 0) return fail(FNI8_ERR_ALIGN, "dequantize_rows_fp4: misaligned out");
   const uintptr_t a = reinterpret_cast<uintptr_t>(out) | (M > 1 ? static_cast<uintptr_t>(K) * esz : 0);
   const int64_t per_row = (K + 7) / 8;
-  const int threads = per_row >= 256 ? 256 : (int)((per_row + 31) / 32 * 32);
-  const dim3 grid((unsigned)(M < 148 * 64 ? M : 148 * 64));
+  // four steps of a row to a thread, so that their loads are in flight together, and 256
+  // threads to a CTA
+  int threads = 32;
+  while (threads < 256 && threads * 4 < per_row) threads *= 2;
+  const int rows = 256 / threads;
+  const int64_t ctas = (M + rows - 1) / rows;
+  const dim3 grid((unsigned)(ctas < 148 * 64 ? ctas : 148 * 64)), block(threads, rows);
 #define FNI8_DEQUANT_FP4(T, FMT, VB) \
-  launch_pdl(fp4::dequant_rows<T, FMT, VB>, grid, dim3(threads), 0, st, q, sf, row_scale, M, K, static_cast<T*>(out))
+  launch_pdl(fp4::dequant_rows<T, FMT, VB>, grid, block, 0, st, q, sf, row_scale, M, K, static_cast<T*>(out))
 #define FNI8_DEQUANT_VB(T, FMT)                          \
   do {                                                   \
     if (a % 16 == 0) FNI8_DEQUANT_FP4(T, FMT, 16);       \
