@@ -72,7 +72,7 @@ static int encode(CUtensorMap* map, const void* base, cuuint32_t rank, const cuu
   for (cuuint32_t i = 0; i + 1 < rank; ++i)
     if (strides[i] % 16 != 0) return fail(FNI8_ERR_ALIGN, "TMA stride %llu not a multiple of 16 bytes",
                                           (unsigned long long)strides[i]);
-  const cuuint32_t estr[3] = {1, 1, 1};
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   CUresult r = fn(map, dt, rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(FNI8_ERR_INVALID, "cuTensorMapEncodeTiled failed (%d)", (int)r);
@@ -93,6 +93,19 @@ int encode_tmap_2d_u8_sw64(CUtensorMap* map, const void* base, uint64_t inner, u
   const cuuint64_t strides[1] = {row_stride_bytes};
   const cuuint32_t box[2] = {box_inner, box_outer};
   return encode(map, base, 2, dims, strides, box, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+int encode_tmap_i8(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                   const uint32_t* box) {
+  if (rank < 2 || rank > 5) return fail(FNI8_ERR_INVALID, "tensor map rank %d", rank);
+  cuuint64_t d[5], st[4];
+  cuuint32_t b[5];
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+    if (i + 1 < rank) st[i] = strides[i];
+  }
+  return encode(map, base, (cuuint32_t)rank, d, st, b, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 int encode_tmap_2d_u8(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t row_stride_bytes,

@@ -129,6 +129,13 @@ struct FewMoe {
   int act;
   void* h;
   void* out;
+  // scratch for the lists that pass from one kernel to the other: [1], 4 x [T k], [T k][16]
+  int32_t* t_count;
+  int32_t* t_slot_e;
+  float* t_slot_w;
+  int32_t* t_ent_e;
+  int32_t* t_ent_n;
+  uint16_t* t_list;
 };
 bool few_supported(int64_t T, int64_t H, int64_t k, int64_t E, int64_t I);
 int few_moe(const FewMoe& m, cudaStream_t st);

@@ -473,6 +473,18 @@ static bool few_tokens(const void* x, int act, int64_t T, int64_t H, int64_t k, 
          few_supported(T, H, k, E, I);
 }
 
+// The two-kernel form's scratch within the composed path's workspace.
+static void few_scratch(FewMoe& m, uint8_t* b) {
+  const MoeLayout L = moe_layout(m.T, m.H, m.k, m.E, m.I);
+  m.h = b + L.h;
+  m.t_count = reinterpret_cast<int32_t*>(b + L.counts);
+  m.t_slot_e = reinterpret_cast<int32_t*>(b + L.ros);
+  m.t_slot_w = reinterpret_cast<float*>(b + L.sor);
+  m.t_ent_e = reinterpret_cast<int32_t*>(b + L.as);
+  m.t_ent_n = reinterpret_cast<int32_t*>(b + L.hs);
+  m.t_list = reinterpret_cast<uint16_t*>(b + L.y);  // 32 bytes per slot, of 2 H
+}
+
 extern "C" int fni8_moe_experts_w8a8(const void* x, int dtype, int64_t T, int64_t H, const int32_t* topi,
                                      const float* topw, int64_t top_k, const int8_t* w_gu, const float* s_gu,
                                      const int8_t* w_dn, const float* s_dn, int64_t E, int64_t I, int act, void* out,
@@ -501,9 +513,12 @@ extern "C" int fni8_moe_experts_w8a8(const void* x, int dtype, int64_t T, int64_
   void* y = b + L.y;
   const int64_t R = T * top_k;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (few_tokens(x, act, T, H, top_k, E, I))
-    return few_moe({x, dtype, T, H, E, I, top_k, nullptr, topi, topw, 0, nullptr, 0, 0, 0, 1.0f, w_gu, s_gu, w_dn, s_dn,
-                    act, h, out}, st);
+  if (few_tokens(x, act, T, H, top_k, E, I)) {
+    FewMoe m{x, dtype, T, H, E, I, top_k, nullptr, topi, topw, 0, nullptr, 0, 0, 0, 1.0f, w_gu, s_gu, w_dn, s_dn, act};
+    m.out = out;
+    few_scratch(m, b);
+    return few_moe(m, st);
+  }
   // plan first (with the segment tables), then each token is quantised once and its int8
   // row written straight to the grouped rows of its slots (no [T, H] int8 copy, no gather)
   if (int s = moe_plan(topi, R, E, counts, offsets, ros, sor, b + L.plan, L.counts - L.plan, tables, stream))
@@ -551,11 +566,13 @@ extern "C" int fni8_moe_layer_w8a8(const void* x, int dtype, int64_t T, int64_t 
   if (workspace == nullptr || workspace_bytes < need)
     return fail(FNI8_ERR_WORKSPACE, "moe needs %zu workspace bytes (got %zu)", need, workspace_bytes);
   if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail(FNI8_ERR_ALIGN, "moe: workspace must be 256-byte aligned");
-  if (few_tokens(x, act, T, H, top_k, E, I))
-    return few_moe({x, dtype, T, H, E, I, top_k, logits, nullptr, nullptr, scoring, sel_bias, n_groups, topk_group,
-                    norm_topk, scaling, w_gu, s_gu, w_dn, s_dn, act,
-                    static_cast<uint8_t*>(workspace) + moe_layout(T, H, top_k, E, I).h, out},
-                   static_cast<cudaStream_t>(stream));
+  if (few_tokens(x, act, T, H, top_k, E, I)) {
+    FewMoe m{x, dtype, T, H, E, I, top_k, logits, nullptr, nullptr, scoring, sel_bias, n_groups, topk_group, norm_topk,
+             scaling, w_gu, s_gu, w_dn, s_dn, act};
+    m.out = out;
+    few_scratch(m, static_cast<uint8_t*>(workspace));
+    return few_moe(m, static_cast<cudaStream_t>(stream));
+  }
   const size_t part = align256(static_cast<size_t>(T) * top_k * 4), base = need - 2 * part;
   int32_t* topi = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + base);
   float* topw = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + base + part);

@@ -22,11 +22,13 @@
 //    no exchange. In few_down a CTA owns 16 output columns through all experts, keeps their
 //    y in shared memory and sums each token's k slots there: no atomics, no third kernel.
 //  * Each CTA routes, quantises the rows and lists the experts for itself (T rows of x, the
-//    T k rows of h): cheaper than a launch that would hand them over. few_down does its
-//    routing and starts its weight loads before it waits for few_gate_up.
+//    T k rows of h): cheaper than a launch that would hand them over. Where both kernels fit
+//    on an SM few_down does that too, and starts its weight loads, before it waits for
+//    few_gate_up; where they do not it reads the lists that few_gate_up leaves.
 //  * Lane (g, q) of a warp reads the 16-byte pieces 2 q + j (j = 0, 1) of row g of a 128-byte
 //    column: with the swizzle, eight neighbouring lanes then touch all 32 banks. The order of
 //    K inside a piece is the same on both sides of the product, so it needs no shuffle.
+#include <mutex>
 #include <type_traits>
 
 #include "fni8_common.cuh"
@@ -60,14 +62,23 @@ struct Layer {
   void* h;            // [T k, I]
   void* out;          // [T, H]
   int stages;
+  // few_down begins before few_gate_up has ended (both fit on an SM) and lists the experts for
+  // itself; else it reads few_gate_up's lists: entries, n, slots' experts and weights.
+  int early;
+  int32_t* t_count;  // [1]
+  int32_t* t_slot_e;
+  float* t_slot_w;
+  int32_t* t_ent_e;
+  int32_t* t_ent_n;
+  uint16_t* t_list;  // [T k][kEntry]
 };
 
 // Shared-memory plan of either kernel: `row` bytes of codes per row (odd multiple of 16 modulo
 // 128, so that rows fall on different banks).
 struct Plan {
-  int row, codes, slot_e, slot_w, scale, ent_e, ent_n, list, extra, bars, total;
+  int row, codes, slot_e, slot_w, scale, ent_e, ent_n, list, masks, extra, bars, total;
 };
-__host__ __device__ inline Plan make_plan(int stages, int rows, int k_len, int slots, int extra_bytes) {
+__host__ __device__ inline Plan make_plan(int stages, int rows, int k_len, int slots, int E, int extra_bytes) {
   Plan p;
   int o = kWarps * stages * kStage;
   auto take = [&](int bytes) {
@@ -83,6 +94,7 @@ __host__ __device__ inline Plan make_plan(int stages, int rows, int k_len, int s
   p.ent_e = take(slots * 4);
   p.ent_n = take(slots * 4);
   p.list = take(slots * kEntry * 2);
+  p.masks = take(E * ((slots + 31) / 32) * 4);
   p.extra = take(extra_bytes);
   p.bars = take(kWarps * 4 * 8);
   p.total = o + 1024;  // the ring is aligned to 1024 bytes
@@ -104,39 +116,132 @@ __device__ __forceinline__ void unpack8(const uint4& u, float (&f)[8]) {
   for (int i = 0; i < 8; ++i) f[i] = to_f32<T>(v[i]);
 }
 
-// One warp: int8 row of src[K] (K a multiple of 16) into dst, zeros up to a multiple of 128;
-// returns the scale. The row is read twice, the second time from L1.
+// Absmax of eight values, NaNs left out (as fmaxf leaves them out).
 template <typename T>
-__device__ __forceinline__ float quant_row(const T* __restrict__ src, int K, uint8_t* dst, int lane) {
-  const uint4* s = reinterpret_cast<const uint4*>(src);
-  const int n = K >> 3;
-  float amax = 0.0f;
-#pragma unroll 4
-  for (int c = lane; c < n; c += 32) {
-    float f[8];
-    unpack8<T>(s[c], f);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(f[i]));
-  }
-  amax = moe::warp_max(amax);
-  const float inv = quant_inv(amax);
-  const int padded = (K + 127) / 128 * 16;
-#pragma unroll 4
-  for (int c = lane; c < padded; c += 32) {
-    uint32_t w[2] = {0u, 0u};
-    if (c < n) {
-      float f[8];
-      unpack8<T>(s[c], f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        w[i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(quant_one(f[i], inv))) << (8 * (i & 3));
-    }
-    *reinterpret_cast<uint2*>(dst + c * 8) = make_uint2(w[0], w[1]);
-  }
-  return quant_scale(amax);
+__device__ __forceinline__ float abs_max8(const uint4& u);
+template <>
+__device__ __forceinline__ float abs_max8<__half>(const uint4& u) {
+  const __half2* h = reinterpret_cast<const __half2*>(&u);
+  const __half2 m = __hmax2(__hmax2(__habs2(h[0]), __habs2(h[1])), __hmax2(__habs2(h[2]), __habs2(h[3])));
+  return __half2float(__hmax(__low2half(m), __high2half(m)));
+}
+template <>
+__device__ __forceinline__ float abs_max8<__nv_bfloat16>(const uint4& u) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+  const __nv_bfloat162 m = __hmax2(__hmax2(__habs2(h[0]), __habs2(h[1])), __hmax2(__habs2(h[2]), __habs2(h[3])));
+  return __bfloat162float(__hmax(__low2bfloat16(m), __high2bfloat16(m)));
 }
 
-__device__ __forceinline__ void route_one(const Layer& p, int t, int lane, int* slot_e, float* slot_w) {
+// quant_one of four values, packed: the clamp comes before the rounding (the same, its bounds
+// are whole), which is an addition of 1.5 * 2^23: the low byte then holds the code.
+__device__ __forceinline__ uint32_t quant4(const float* f, float inv) {
+  uint32_t b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float t = fminf(fmaxf(__fmul_rn(f[i], inv), -127.0f), 127.0f);
+    b[i] = __float_as_uint(__fadd_rn(t, 12582912.0f));
+  }
+  return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+}
+
+// A value into this CTA's shared memory and the same place in its cluster peers'.
+template <typename V>
+__device__ __forceinline__ void share(V* at, V v, int peers) {
+  static_assert(sizeof(V) == 4 || sizeof(V) == 8, "words");
+  if (peers == 1) {
+    *at = v;
+    return;
+  }
+  const uint32_t local = smem_u32(at);
+  for (int p = 0; p < peers; ++p) {
+    const uint32_t to = mapa_shared(local, static_cast<uint32_t>(p));
+    if constexpr (sizeof(V) == 8) {
+      const uint2 w = *reinterpret_cast<const uint2*>(&v);
+      asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(to), "r"(w.x), "r"(w.y) : "memory");
+    } else {
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(*reinterpret_cast<const uint32_t*>(&v)) : "memory");
+    }
+  }
+}
+
+// Every thread of the CTA, or of the cluster: what they shared before is seen after.
+__device__ __forceinline__ void join(int peers) {
+  __syncwarp();
+  if (peers > 1) cluster_sync_all();
+  else __syncthreads();
+}
+
+// One warp: int8 rows i0, i0 + step, ... (R of them, those below n) of src [n, K] (K a multiple
+// of 16) into dst [n][row_bytes], zeros up to a multiple of 128, and their scales, here and in
+// the cluster's other CTAs. C: 256-value pieces of a row that the warp keeps in registers
+// (0: a longer row, read twice).
+template <typename T, int R, int C>
+__device__ __forceinline__ void quant_rows(const T* __restrict__ src, int n, int K, int i0, int step, uint8_t* dst,
+                                           int row_bytes, float* scale, int lane, int peers) {
+  const int nc = K >> 3, padded = (K + 127) / 128 * 16;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  const uint4* s[R];
+  uint4 raw[R][C > 0 ? C : 1];
+  float amax[R], inv[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    s[r] = reinterpret_cast<const uint4*>(src + static_cast<int64_t>(min(i0 + r * step, n - 1)) * K);
+    amax[r] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) raw[r][c] = lane + c * 32 < nc ? s[r][lane + c * 32] : zero;
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if constexpr (C > 0) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) amax[r] = fmaxf(amax[r], abs_max8<T>(raw[r][c]));
+    } else {
+#pragma unroll 8
+      for (int c = lane; c < nc; c += 32) amax[r] = fmaxf(amax[r], abs_max8<T>(s[r][c]));
+    }
+    amax[r] = moe::warp_max(amax[r]);
+    inv[r] = quant_inv(amax[r]);
+    const int i = i0 + r * step;
+    if (lane == 0 && i < n) share(scale + i, quant_scale(amax[r]), peers);
+  }
+  auto put = [&](int r, int c, const uint4& u) {
+    float f[8];
+    unpack8<T>(u, f);
+    uint2 w = make_uint2(quant4(f, inv[r]), quant4(f + 4, inv[r]));
+    if (c >= nc) w = make_uint2(0u, 0u);  // (an infinite or NaN factor makes no zero of a zero)
+    const int i = i0 + r * step;
+    if (i < n && c < padded) share(reinterpret_cast<uint2*>(dst + i * row_bytes + c * 8), w, peers);
+  };
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if constexpr (C > 0) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        if (c * 32 < padded) put(r, lane + c * 32, raw[r][c]);
+    } else {
+#pragma unroll 4
+      for (int c = lane; c < padded; c += 32) put(r, c, c < nc ? s[r][c] : zero);
+    }
+  }
+}
+
+// All rows of src [n, K], dealt out to the warps of the cluster's CTAs, R at a time.
+template <typename T, int R>
+__device__ __forceinline__ void quant_all(const T* __restrict__ src, int n, int K, int worker, int workers, uint8_t* dst,
+                                          int row_bytes, float* scale, int lane, int peers) {
+  if (K <= 1024) {
+    for (int i = worker; i < n; i += R * workers)
+      quant_rows<T, R, 4>(src, n, K, i, workers, dst, row_bytes, scale, lane, peers);
+  } else if (K <= 2048) {
+    for (int i = worker; i < n; i += workers)
+      quant_rows<T, 1, 8>(src, n, K, i, workers, dst, row_bytes, scale, lane, peers);
+  } else {
+    for (int i = worker; i < n; i += workers)
+      quant_rows<T, 1, 0>(src, n, K, i, workers, dst, row_bytes, scale, lane, peers);
+  }
+}
+
+__device__ __forceinline__ void route_one(const Layer& p, int t, int lane, int* slot_e, float* slot_w, int peers) {
   const float* lr = p.logits + static_cast<int64_t>(t) * p.E;
   int e = 0;
   float w = 0.0f;
@@ -150,63 +255,78 @@ __device__ __forceinline__ void route_one(const Layer& p, int t, int lane, int* 
   else if (p.E <= 256) go(std::integral_constant<int, 8>{});
   else go(std::integral_constant<int, 16>{});
   if (lane < p.k) {
-    slot_e[t * p.k + lane] = e;
-    slot_w[t * p.k + lane] = w;
+    share(slot_e + t * p.k + lane, e, peers);
+    share(slot_w + t * p.k + lane, w, peers);
   }
 }
 
 // Entries: the slots of each expert, at most kEntry to an entry (an id that appears more often
-// has several), slots in order. A slot whose id is outside [0, E) is in none. Returns their
-// number; every thread of the CTA takes part. Quadratic in the slots, which are few.
-__device__ int list_entries(const int* slot_e, int n, int E, int* ent_e, int* ent_n, uint16_t* list) {
+// has several), slots in order. A slot whose id is outside [0, E) is in none. masks: for each
+// expert the slots that name it, a bit each. Returns the number of entries; every thread of
+// the CTA takes part.
+__device__ int list_entries(const int* slot_e, int n, int E, int* ent_e, int* ent_n, uint16_t* list, uint32_t* masks) {
   __shared__ int warp_sum[2 * kWarps];
-  __shared__ int16_t ent_of[kMaxSlots];
+  __shared__ int16_t ent_of[kMaxSlots];  // of an entry's first slot
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int base = 0, rank[2], start[2];
+  const int words = (n + 31) >> 5;
+  for (int i = threadIdx.x; i < E * words; i += kThreads) masks[i] = 0u;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const int e = slot_e[i];
+    if (e >= 0 && e < E) atomicOr(&masks[e * words + (i >> 5)], 1u << (i & 31));
+  }
+  __syncthreads();
+  static_assert(kMaxSlots <= 2 * kThreads, "two slots to a thread");
+  int total = 0, rank[2] = {-1, -1};
+#pragma unroll
   for (int r = 0; r < 2; ++r) {
-    const int i = r * kThreads + threadIdx.x;
-    const int e = i < n ? slot_e[i] : -1;
-    const bool valid = e >= 0 && e < E;
-    int before = 0, first = i, all = 0;
-    if (valid) {
-      for (int j = 0; j < n; ++j) {
-        if (slot_e[j] == e) {
-          if (j < i) {
-            if (before % kEntry == 0) first = j;
-            ++before;
-          }
-          ++all;
+    if (r * kThreads < n) {
+      const int i = r * kThreads + threadIdx.x;
+      const int e = i < n ? slot_e[i] : -1;
+      int before = -1, all = 0;
+      if (e >= 0 && e < E) {
+        before = 0;
+        for (int w = 0; w < words; ++w) {
+          const uint32_t m = masks[e * words + w];
+          const int bit = i - w * 32;
+          before += __popc(bit >= 32 ? m : bit <= 0 ? 0u : m & ((1u << bit) - 1u));
+          all += __popc(m);
         }
       }
-      if (before % kEntry == 0) first = i;
+      rank[r] = before;
+      const bool opens = before >= 0 && before % kEntry == 0;
+      const unsigned m = __ballot_sync(0xffffffffu, opens);
+      if (lane == 0) warp_sum[r * kWarps + warp] = __popc(m);
+      __syncthreads();
+      int at = total;
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) at += warp_sum[r * kWarps + w];
+        total += warp_sum[r * kWarps + w];
+      }
+      if (opens) {
+        const int a = at + __popc(m & ((1u << lane) - 1u));
+        ent_of[i] = static_cast<int16_t>(a);
+        ent_e[a] = e;
+        ent_n[a] = min(kEntry, all - before);
+      }
     }
-    rank[r] = valid ? before : -1;
-    start[r] = first;
-    const bool opens = valid && before % kEntry == 0;
-    const unsigned m = __ballot_sync(0xffffffffu, opens);
-    if (lane == 0) warp_sum[r * kWarps + warp] = __popc(m);
-    __syncthreads();
-    int at = base;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) at += warp_sum[r * kWarps + w];
-      base += warp_sum[r * kWarps + w];
-    }
-    if (opens) {
-      const int a = at + __popc(m & ((1u << lane) - 1u));
-      ent_of[i] = static_cast<int16_t>(a);
-      ent_e[a] = e;
-      ent_n[a] = min(kEntry, all - before);
-    }
-    if (n <= kThreads) break;
   }
   __syncthreads();
+#pragma unroll
   for (int r = 0; r < 2; ++r) {
-    const int i = r * kThreads + threadIdx.x;
-    if (i < n && rank[r] >= 0) list[ent_of[start[r]] * kEntry + rank[r] % kEntry] = static_cast<uint16_t>(i);
-    if (n <= kThreads) break;
+    if (rank[r] >= 0) {
+      // the entry's first slot: the one of rank [rank / kEntry] * kEntry
+      const int i = r * kThreads + threadIdx.x;
+      const uint32_t* mk = masks + slot_e[i] * words;
+      int left = rank[r] / kEntry * kEntry, w = 0;
+      while (left >= __popc(mk[w])) left -= __popc(mk[w++]);
+      uint32_t bits = mk[w];
+      for (; left > 0; --left) bits &= bits - 1u;
+      list[ent_of[w * 32 + __ffs(bits) - 1] * kEntry + rank[r] % kEntry] = static_cast<uint16_t>(i);
+    }
   }
   __syncthreads();
-  return base;
+  return total;
 }
 
 // One stage (16 weight rows x 256 bytes from k0 on, in two 128-byte columns; none behind K)
@@ -233,12 +353,12 @@ __device__ __forceinline__ void stage_product(int (&acc)[NT][4], const uint8_t* 
   }
 }
 
-template <typename T, int ACT>
+template <typename T, int ACT, bool WIDE>
 __global__ void __launch_bounds__(kThreads) few_gate_up(const __grid_constant__ CUtensorMap tmW, Layer p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int n = p.T * p.k;
-  const Plan pl = make_plan(p.stages, p.T, p.H, n, 0);
+  const Plan pl = make_plan(p.stages, p.T, p.H, n, p.E, 0);
   uint8_t* codes = smem + pl.codes;
   int* slot_e = reinterpret_cast<int*>(smem + pl.slot_e);
   float* slot_w = reinterpret_cast<float*>(smem + pl.slot_w);
@@ -254,21 +374,33 @@ __global__ void __launch_bounds__(kThreads) few_gate_up(const __grid_constant__ 
     for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1);
     fence_barrier_init();
   }
+  const int rank = static_cast<int>(cluster_ctarank()), peers = static_cast<int>(cluster_nctarank());
+  const int workers = peers * kWarps;
+  if (peers > 1) cluster_sync_all();  // the peers have started
   pdl_wait();
-  const int routes = p.logits != nullptr ? p.T : 0;
-  if (routes == 0)
+  // routing on the first warps of every CTA, the rows on the last, so that both run at once
+  if (p.logits != nullptr) {
+    for (int t = warp * peers + rank; t < p.T; t += workers) route_one(p, t, lane, slot_e, slot_w, peers);
+  } else {
     for (int i = threadIdx.x; i < n; i += kThreads) slot_e[i] = p.topi[i];
-  for (int job = warp; job < routes + p.T; job += kWarps) {
-    if (job < routes) {
-      route_one(p, job, lane, slot_e, slot_w);
-    } else {
-      const int t = job - routes;
-      const float s = quant_row<T>(static_cast<const T*>(p.x) + static_cast<int64_t>(t) * p.H, p.H, codes + t * pl.row, lane);
-      if (lane == 0) a_s[t] = s;
-    }
   }
-  __syncthreads();
-  const int n_ent = list_entries(slot_e, n, p.E, ent_e, ent_n, list);
+  quant_all<T, 1>(static_cast<const T*>(p.x), p.T, p.H, (kWarps - 1 - warp) * peers + rank, workers, codes, pl.row, a_s,
+                  lane, peers);
+  join(peers);
+  const int n_ent = list_entries(slot_e, n, p.E, ent_e, ent_n, list, reinterpret_cast<uint32_t*>(smem + pl.masks));
+
+  if (!p.early && blockIdx.x == 0) {  // hand the lists over
+    if (threadIdx.x == 0) *p.t_count = n_ent;
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      p.t_slot_e[i] = slot_e[i];
+      p.t_slot_w[i] = p.logits != nullptr ? slot_w[i] : p.topw[i];
+      p.t_ent_e[i] = ent_e[i];
+      p.t_ent_n[i] = ent_n[i];
+    }
+    for (int i = threadIdx.x; i < n * kEntry / 2; i += kThreads)
+      reinterpret_cast<uint32_t*>(p.t_list)[i] = reinterpret_cast<const uint32_t*>(list)[i];
+  }
+  pdl_launch_dependents();
 
   const int U = p.I >> 3, KC = (p.H + 255) >> 8;
   const int first = warp * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x);
@@ -276,27 +408,38 @@ __global__ void __launch_bounds__(kThreads) few_gate_up(const __grid_constant__ 
   const int total = n_ent * U;
   const int units = total > first ? (total - first - 1) / stride + 1 : 0;
   const int steps = units * KC;
-  int pu = first, pk = 0, ps = 0;  // the next stage to load (lane 0)
+  // the next stage to load (lane 0): unit pu = entry pa, column block pc
+  int pu = first, pa = first / U, pc = first % U, pk = 0, ps = 0;
+  const int stride_a = stride / U, stride_c = stride % U;
+  const uint64_t policy = evict_first_policy();
   auto issue = [&]() {
     uint8_t* dst = ring + ps * kStage;
     uint64_t* bar = &full[ps];
-    const int e = ent_e[pu / U], c = pu % U * 8;
+    const int e = ent_e[pa], c = pc * 8;
     mbar_arrive_expect_tx(bar, kStage);
+    if constexpr (WIDE) {  // 128 bytes x 8 rows x {gate, up} x 2 columns
+      tma_load_5d(&tmW, bar, dst, 0, c, 0, pk * 2, e, policy);
+    } else {
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      tma_load_3d(&tmW, bar, dst + hh * 2048, pk * 256 + hh * 128, c, e);
-      tma_load_3d(&tmW, bar, dst + hh * 2048 + 1024, pk * 256 + hh * 128, p.I + c, e);
+      for (int hh = 0; hh < 2; ++hh) {
+        tma_load_3d(&tmW, bar, dst + hh * 2048, pk * 256 + hh * 128, c, e, policy);
+        tma_load_3d(&tmW, bar, dst + hh * 2048 + 1024, pk * 256 + hh * 128, p.I + c, e, policy);
+      }
     }
     if (++pk == KC) {
       pk = 0;
       pu += stride;
+      pa += stride_a;
+      if ((pc += stride_c) >= U) {
+        pc -= U;
+        ++pa;
+      }
     }
     if (++ps == p.stages) ps = 0;
   };
   int issued = min(steps, p.stages), consumed = 0;
   if (lane == 0)
     for (int i = 0; i < issued; ++i) issue();
-  pdl_launch_dependents();
 
   int s = 0;
   uint32_t ph = 0;
@@ -363,12 +506,12 @@ __global__ void __launch_bounds__(kThreads) few_gate_up(const __grid_constant__ 
   }
 }
 
-template <typename T>
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kThreads) few_down(const __grid_constant__ CUtensorMap tmW, Layer p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int n = p.T * p.k;
-  const Plan pl = make_plan(p.stages, n, p.I, n, n * 64);
+  const Plan pl = make_plan(p.stages, n, p.I, n, p.E, n * 64);
   uint8_t* codes = smem + pl.codes;
   int* slot_e = reinterpret_cast<int*>(smem + pl.slot_e);
   float* slot_w = reinterpret_cast<float*>(smem + pl.slot_w);
@@ -385,30 +528,53 @@ __global__ void __launch_bounds__(kThreads) few_down(const __grid_constant__ CUt
     for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1);
     fence_barrier_init();
   }
-  // The routing's inputs are older than few_gate_up, which released this kernel after its own
-  // wait for them: they are read before this kernel waits for few_gate_up.
-  if (p.logits != nullptr) {
-    for (int t = warp; t < p.T; t += kWarps) route_one(p, t, lane, slot_e, slot_w);
-  } else {
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      slot_e[i] = p.topi[i];
-      slot_w[i] = p.topw[i];
+  const int rank = static_cast<int>(cluster_ctarank()), peers = static_cast<int>(cluster_nctarank());
+  const int workers = peers * kWarps;
+  if (peers > 1) cluster_sync_all();  // the peers have started
+  int n_ent;
+  if (p.early) {
+    // The routing's inputs are older than few_gate_up, which released this kernel after its own
+    // wait for them: they are read before this kernel waits for few_gate_up.
+    if (p.logits != nullptr) {
+      for (int t = warp * peers + rank; t < p.T; t += workers) route_one(p, t, lane, slot_e, slot_w, peers);
+    } else {
+      for (int i = threadIdx.x; i < n; i += kThreads) {
+        slot_e[i] = p.topi[i];
+        slot_w[i] = p.topw[i];
+      }
     }
+    join(peers);
+    n_ent = list_entries(slot_e, n, p.E, ent_e, ent_n, list, reinterpret_cast<uint32_t*>(smem + pl.masks));
+  } else {
+    pdl_wait();
+    n_ent = *p.t_count;
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      slot_e[i] = p.t_slot_e[i];
+      slot_w[i] = p.t_slot_w[i];
+      ent_e[i] = p.t_ent_e[i];
+      ent_n[i] = p.t_ent_n[i];
+    }
+    for (int i = threadIdx.x; i < n * kEntry / 2; i += kThreads)
+      reinterpret_cast<uint32_t*>(list)[i] = reinterpret_cast<const uint32_t*>(p.t_list)[i];
+    __syncthreads();
   }
-  __syncthreads();
-  const int n_ent = list_entries(slot_e, n, p.E, ent_e, ent_n, list);
 
   const int KC = (p.I + 255) >> 8, tiles = p.H >> 4;
-  const int my_tiles = (tiles - static_cast<int>(blockIdx.x) - 1) / static_cast<int>(gridDim.x) + 1;
+  const int my_tiles = (tiles - static_cast<int>(blockIdx.x) - 1 + static_cast<int>(gridDim.x)) / static_cast<int>(gridDim.x);
   const int my_ents = n_ent > warp ? (n_ent - warp - 1) / kWarps + 1 : 0;
   const int steps = my_tiles * my_ents * KC;
   int pt = static_cast<int>(blockIdx.x), pa = warp, pk = 0, ps = 0;
+  const uint64_t policy = evict_first_policy();
   auto issue = [&]() {
     uint8_t* dst = ring + ps * kStage;
     uint64_t* bar = &full[ps];
     mbar_arrive_expect_tx(bar, kStage);
-    tma_load_3d(&tmW, bar, dst, pk * 256, pt * 16, ent_e[pa]);
-    tma_load_3d(&tmW, bar, dst + 2048, pk * 256 + 128, pt * 16, ent_e[pa]);
+    if constexpr (WIDE) {  // 128 bytes x 16 rows x 2 columns
+      tma_load_4d(&tmW, bar, dst, 0, pt * 16, pk * 2, ent_e[pa], policy);
+    } else {
+      tma_load_3d(&tmW, bar, dst, pk * 256, pt * 16, ent_e[pa], policy);
+      tma_load_3d(&tmW, bar, dst + 2048, pk * 256 + 128, pt * 16, ent_e[pa], policy);
+    }
     if (++pk == KC) {
       pk = 0;
       if ((pa += kWarps) >= n_ent) {
@@ -422,11 +588,8 @@ __global__ void __launch_bounds__(kThreads) few_down(const __grid_constant__ CUt
   if (lane == 0)
     for (int i = 0; i < issued; ++i) issue();
   pdl_wait();
-  for (int i = warp; i < n; i += kWarps) {
-    const float sc = quant_row<T>(static_cast<const T*>(p.h) + static_cast<int64_t>(i) * p.I, p.I, codes + i * pl.row, lane);
-    if (lane == 0) h_s[i] = sc;
-  }
-  __syncthreads();
+  quant_all<T, 2>(static_cast<const T*>(p.h), n, p.I, warp * peers + rank, workers, codes, pl.row, h_s, lane, peers);
+  join(peers);
   pdl_launch_dependents();
 
   int s = 0;
@@ -522,13 +685,64 @@ int few_status_read_and_clear(int* code) {
 
 namespace {
 
+#ifndef FEW_MIN
+#define FEW_MIN 24
+#endif
 constexpr int kSmemMax = 226 * 1024;  // static shared memory (the entry list's) beside it
 
 // Ring depth of a kernel: three stages a warp, two where the codes leave no room; 0: none fits.
-int few_stages(int rows, int64_t k_len, int slots, int extra) {
+int few_stages(int rows, int64_t k_len, int slots, int E, int extra) {
   for (int st = 3; st >= 2; --st)
-    if (few::make_plan(st, rows, (int)k_len, slots, extra).total + 2048 <= kSmemMax) return st;
+    if (few::make_plan(st, rows, (int)k_len, slots, E, extra).total + 2048 <= kSmemMax) return st;
   return 0;
+}
+
+// CTAs per cluster that share the preparation: with few rows it costs more than it saves.
+int few_cluster(int64_t rows) { return rows >= FEW_MIN ? 8 : 1; }
+
+// Grid of `want` CTAs at most, in clusters of cs that are resident at once.
+int few_grid(int64_t want, int smem, int cs) {
+  const int sms = num_sms(current_device());
+  int64_t n = want < sms ? want : sms;
+  if (cs > 1) {
+    struct Entry { int dev, smem, n; };
+    static Entry cache[64];
+    static int used = 0;
+    static std::mutex mu;
+    std::lock_guard<std::mutex> lock(mu);
+    const int dev = current_device();
+    int most = -1;
+    for (int i = 0; i < used; ++i)
+      if (cache[i].dev == dev && cache[i].smem == smem) most = cache[i].n;
+    if (most < 0) {
+      most = max_active_clusters(few::kThreads, smem, cs);
+      if (most >= 0 && used < 64) cache[used++] = Entry{dev, smem, most};
+    }
+    if (most < 1) most = sms / cs;
+    n = (n + cs - 1) / cs;
+    n = (n < most ? n : most) * cs;
+  }
+  return (int)n;
+}
+
+template <typename... KArgs, typename... Args>
+void launch_cluster(void (*kern)(KArgs...), int grid, int cs, int smem, cudaStream_t st, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(few::kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled();
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cs;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+  if (e != cudaSuccess && t_launch_error == cudaSuccess) t_launch_error = e;
 }
 
 template <typename Kern>
@@ -536,27 +750,52 @@ int configure(Kern kern, std::atomic<bool>* done) {
   const int dev = current_device();
   if (dev < 0 || dev >= kMaxDevices) return fail(FNI8_ERR_CUDA, "no current CUDA device");
   if (done[dev]) return FNI8_OK;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax - 2048);
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax - 2048);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
   if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(few-token layer)");
   done[dev] = true;
   return FNI8_OK;
 }
 
-template <typename T, int ACT>
-int launch_few(few::Layer& p, const CUtensorMap& gu, const CUtensorMap& dn, cudaStream_t st) {
-  static std::atomic<bool> done_a[kMaxDevices] = {}, done_b[kMaxDevices] = {};
-  if (int s = configure(few::few_gate_up<T, ACT>, done_a)) return s;
-  if (int s = configure(few::few_down<T>, done_b)) return s;
-  const int sms = num_sms(current_device());
+template <typename T, int ACT, bool WIDE_GU>
+int launch_gate_up(const few::Layer& p, const CUtensorMap& map, int smem, cudaStream_t st) {
+  static std::atomic<bool> done[kMaxDevices] = {};
+  if (int s = configure(few::few_gate_up<T, ACT, WIDE_GU>, done)) return s;
+  const int cs = few_cluster(p.T * p.k);
+  // units at most: every slot its own expert
+  const int grid = few_grid((int64_t)p.T * p.k * (p.I / 8), smem, cs);
+  launch_cluster(few::few_gate_up<T, ACT, WIDE_GU>, grid, cs, smem, st, map, p);
+  return FNI8_OK;
+}
+
+template <typename T, bool WIDE_DN>
+int launch_down(const few::Layer& p, const CUtensorMap& map, int smem, cudaStream_t st) {
+  static std::atomic<bool> done[kMaxDevices] = {};
+  if (int s = configure(few::few_down<T, WIDE_DN>, done)) return s;
+  const int cs = few_cluster(p.T * p.k);
+  launch_cluster(few::few_down<T, WIDE_DN>, few_grid(p.H / 16, smem, cs), cs, smem, st, map, p);
+  return FNI8_OK;
+}
+
+template <typename T>
+int launch_few(const few::Layer& layer, int act, const CUtensorMap& gu, const CUtensorMap& dn, cudaStream_t st) {
+  few::Layer p = layer, d = layer;
   const int slots = p.T * p.k;
-  p.stages = few_stages(p.T, p.H, slots, 0);
-  const int64_t most = (int64_t)slots * (p.I / 8);  // units, if every slot had its own expert
-  launch_pdl(few::few_gate_up<T, ACT>, dim3((unsigned)(most < sms ? most : sms)), dim3(few::kThreads),
-             few::make_plan(p.stages, p.T, p.H, slots, 0).total, st, gu, p);
-  p.stages = few_stages(slots, p.I, slots, slots * 64);
-  const int tiles = p.H / 16;
-  launch_pdl(few::few_down<T>, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(few::kThreads),
-             few::make_plan(p.stages, slots, p.I, slots, slots * 64).total, st, dn, p);
+  p.stages = few_stages(p.T, p.H, slots, p.E, 0);
+  d.stages = few_stages(slots, p.I, slots, p.E, slots * 64);
+  const int sg = few::make_plan(p.stages, p.T, p.H, slots, p.E, 0).total;
+  const int sd = few::make_plan(d.stages, slots, p.I, slots, p.E, slots * 64).total;
+  p.early = d.early = sg + sd + 2 * 2048 <= kSmemMax ? 1 : 0;
+  const bool wide_gu = p.H % 128 == 0, wide_dn = p.I % 128 == 0;
+  int s;
+  if (act == FNI8_ACT_SILU)
+    s = wide_gu ? launch_gate_up<T, FNI8_ACT_SILU, true>(p, gu, sg, st) : launch_gate_up<T, FNI8_ACT_SILU, false>(p, gu, sg, st);
+  else
+    s = wide_gu ? launch_gate_up<T, FNI8_ACT_GELU_TANH, true>(p, gu, sg, st)
+                : launch_gate_up<T, FNI8_ACT_GELU_TANH, false>(p, gu, sg, st);
+  if (s) return s;
+  if ((s = wide_dn ? launch_down<T, true>(d, dn, sd, st) : launch_down<T, false>(d, dn, sd, st))) return s;
   FNI8_CHECK_LAUNCH("moe few-token layer");
   return FNI8_OK;
 }
@@ -567,25 +806,32 @@ bool few_supported(int64_t T, int64_t H, int64_t k, int64_t E, int64_t I) {
   if (T < 1 || T > few::kMaxTokens || k < 1 || k > 32 || T * k > few::kMaxSlots || E < 1 || E > 512) return false;
   if (H % 16 != 0 || I % 16 != 0 || H > (1 << 17) || I > (1 << 17)) return false;
   const int n = (int)(T * k);
-  return few_stages((int)T, H, n, 0) > 0 && few_stages(n, I, n, n * 64) > 0;
+  return few_stages((int)T, H, n, (int)E, 0) > 0 && few_stages(n, I, n, (int)E, n * 64) > 0;
 }
 
 int few_moe(const FewMoe& m, cudaStream_t st) {
+  // One load per stage where K is whole 128-byte columns (they become a dimension of the map);
+  // small loads are issued at one in some 35 cycles, four to a stage took the first ring 1.7 us.
   CUtensorMap gu, dn;
-  if (int s = encode_tmap_3d_i8(&gu, m.w_gu, (uint64_t)m.H, (uint64_t)(2 * m.I), (uint64_t)m.E, (uint64_t)m.H,
-                                (uint64_t)(2 * m.I * m.H), 128, 8))
+  const uint64_t H = (uint64_t)m.H, I = (uint64_t)m.I, E = (uint64_t)m.E;
+  if (m.H % 128 == 0) {
+    const uint64_t dims[5] = {128, I, 2, H / 128, E}, strides[4] = {H, I * H, 128, 2 * I * H};
+    const uint32_t box[5] = {128, 8, 2, 2, 1};
+    if (int s = encode_tmap_i8(&gu, m.w_gu, 5, dims, strides, box)) return s;
+  } else if (int s = encode_tmap_3d_i8(&gu, m.w_gu, H, 2 * I, E, H, 2 * I * H, 128, 8)) {
     return s;
-  if (int s = encode_tmap_3d_i8(&dn, m.w_dn, (uint64_t)m.I, (uint64_t)m.H, (uint64_t)m.E, (uint64_t)m.I,
-                                (uint64_t)(m.H * m.I), 128, 16))
-    return s;
-  few::Layer p{m.x, m.logits, m.topi, m.topw, m.sel_bias, (int)m.T, (int)m.H, (int)m.E, (int)m.I, (int)m.k, m.scoring,
-               (int)m.n_groups, (int)m.topk_group, m.norm_topk, m.dtype, m.scaling, m.s_gu, m.s_dn, m.h, m.out, 0};
-  if (m.dtype == FNI8_F16) {
-    if (m.act == FNI8_ACT_SILU) return launch_few<__half, FNI8_ACT_SILU>(p, gu, dn, st);
-    return launch_few<__half, FNI8_ACT_GELU_TANH>(p, gu, dn, st);
   }
-  if (m.act == FNI8_ACT_SILU) return launch_few<__nv_bfloat16, FNI8_ACT_SILU>(p, gu, dn, st);
-  return launch_few<__nv_bfloat16, FNI8_ACT_GELU_TANH>(p, gu, dn, st);
+  if (m.I % 128 == 0) {
+    const uint64_t dims[4] = {128, H, I / 128, E}, strides[3] = {I, 128, H * I};
+    const uint32_t box[4] = {128, 16, 2, 1};
+    if (int s = encode_tmap_i8(&dn, m.w_dn, 4, dims, strides, box)) return s;
+  } else if (int s = encode_tmap_3d_i8(&dn, m.w_dn, I, H, E, I, H * I, 128, 16)) {
+    return s;
+  }
+  few::Layer p{m.x, m.logits, m.topi, m.topw, m.sel_bias, (int)m.T, (int)m.H, (int)m.E, (int)m.I, (int)m.k, m.scoring,
+               (int)m.n_groups, (int)m.topk_group, m.norm_topk, m.dtype, m.scaling, m.s_gu, m.s_dn, m.h, m.out, 0, 0, m.t_count, m.t_slot_e, m.t_slot_w, m.t_ent_e,
+               m.t_ent_n, m.t_list};
+  return m.dtype == FNI8_F16 ? launch_few<__half>(p, m.act, gu, dn, st) : launch_few<__nv_bfloat16>(p, m.act, gu, dn, st);
 }
 
 }  // namespace fni8h

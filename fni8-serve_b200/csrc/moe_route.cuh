@@ -16,17 +16,18 @@ __device__ __forceinline__ float warp_sum(float v) {
   for (int o = 16; o > 0; o >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
-// warp-wide arg-max: larger value wins, ties go to the lower index
+// Order-preserving key of a float that is no NaN (-0 and +0 alike).
+__device__ __forceinline__ uint32_t order_key(float v) {
+  const uint32_t b = __float_as_uint(__fadd_rn(v, 0.0f));
+  return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+// warp-wide arg-max over indexes >= 0: the larger value wins, ties go to the lower index (two
+// warp reductions; a shuffle tree over value and index took three times as long)
 __device__ __forceinline__ void warp_argmax(float& v, int& i) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float ov = __shfl_xor_sync(0xffffffffu, v, o);
-    const int oi = __shfl_xor_sync(0xffffffffu, i, o);
-    if (ov > v || (ov == v && oi < i)) {
-      v = ov;
-      i = oi;
-    }
-  }
+  const uint32_t key = order_key(v);
+  const uint32_t top = __reduce_max_sync(0xffffffffu, key);
+  i = static_cast<int>(__reduce_min_sync(0xffffffffu, key == top ? static_cast<uint32_t>(i) : 0x7fffffffu));
+  v = __uint_as_float((top & 0x80000000u) ? top & 0x7FFFFFFFu : ~top);
 }
 
 // Scores of logits row `lr` [E] and the top k of them: lane j < k returns slot j's expert in
@@ -70,32 +71,33 @@ __device__ __forceinline__ void route_token(const float* __restrict__ lr, int E,
     }
   }
   if (n_groups > 0 && topk_group > 0) {
-    // keep only the topk_group groups with the largest max score
+    // keep only the topk_group groups with the largest max score: lane g takes group g's
+    // maximum, then one arg-max per kept group (a group without a score above -inf is none)
     const int epg = E / n_groups;
+    int group[VPL];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) group[i] = (lane + 32 * i) / epg;
+    float mine = NEG;
+    for (int g = 0; g < n_groups; ++g) {
+      float gm = NEG;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (lane + 32 * i < E && group[i] == g) gm = fmaxf(gm, sel[i]);
+      gm = warp_max(gm);
+      if (lane == g) mine = gm;
+    }
     unsigned keep = 0;  // bitmask over groups (n_groups <= 32)
     for (int r = 0; r < topk_group; ++r) {
-      float best = NEG;
-      int bg = 0x7fffffff;
-      for (int g = 0; g < n_groups; ++g) {
-        if (keep & (1u << g)) continue;
-        float gm = NEG;
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) {
-          const int e = lane + 32 * i;
-          if (e < E && e / epg == g) gm = fmaxf(gm, sel[i]);
-        }
-        gm = warp_max(gm);
-        if (gm > best) {
-          best = gm;
-          bg = g;
-        }
-      }
+      const bool open = lane < n_groups && !(keep & (1u << lane)) && mine > NEG;
+      float best = open ? mine : NEG;
+      int bg = open ? lane : 0x7fffffff;
+      warp_argmax(best, bg);
       if (bg != 0x7fffffff) keep |= 1u << bg;
     }
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
       const int e = lane + 32 * i;
-      if (e < E && !(keep & (1u << (e / epg)))) sel[i] = NEG;
+      if (e < E && !(keep & (1u << group[i]))) sel[i] = NEG;
     }
   }
   float my_w = 0.0f;
