@@ -25,6 +25,10 @@
 //    T k rows of h): cheaper than a launch that would hand them over. Where both kernels fit
 //    on an SM few_down does that too, and starts its weight loads, before it waits for
 //    few_gate_up; where they do not it reads the lists that few_gate_up leaves.
+//  * A CTA runs most of its code once, and an instruction line that is not in its SM's caches
+//    costs 0.1 us and more; so the preparation is short loops, not unrolled ones (listing the
+//    experts of one token: 4.9 us at first sight, 0.8 us the second time), and the weights pass
+//    through L2 with an evict-first policy, which leaves the instructions there.
 //  * Lane (g, q) of a warp reads the 16-byte pieces 2 q + j (j = 0, 1) of row g of a 128-byte
 //    column: with the swizzle, eight neighbouring lanes then touch all 32 banks. The order of
 //    K inside a piece is the same on both sides of the product, so it needs no shuffle.
@@ -44,6 +48,7 @@ constexpr int kStage = 4096;  // 16 weight rows x 256 bytes
 constexpr int kEntry = 16;    // slots of one expert in one entry (two n8 tiles)
 constexpr int kMaxTokens = 16;
 constexpr int kMaxSlots = 512;
+constexpr int kMaxExperts = 512;
 
 static __device__ int g_status;
 enum : int { kCodeGateUp = 0x801, kCodeDown = 0x802 };
@@ -76,7 +81,7 @@ struct Layer {
 // Shared-memory plan of either kernel: `row` bytes of codes per row (odd multiple of 16 modulo
 // 128, so that rows fall on different banks).
 struct Plan {
-  int row, codes, slot_e, slot_w, scale, ent_e, ent_n, list, masks, extra, bars, total;
+  int row, codes, slot_e, slot_w, scale, top, ent_e, ent_n, list, masks, extra, bars, total;
 };
 __host__ __device__ inline Plan make_plan(int stages, int rows, int k_len, int slots, int E, int extra_bytes) {
   Plan p;
@@ -91,6 +96,7 @@ __host__ __device__ inline Plan make_plan(int stages, int rows, int k_len, int s
   p.slot_e = take(slots * 4);
   p.slot_w = take(slots * 4);
   p.scale = take(rows * 4);
+  p.top = take(rows * 4);
   p.ent_e = take(slots * 4);
   p.ent_n = take(slots * 4);
   p.list = take(slots * kEntry * 2);
@@ -171,74 +177,65 @@ __device__ __forceinline__ void join(int peers) {
   else __syncthreads();
 }
 
-// One warp: int8 rows i0, i0 + step, ... (R of them, those below n) of src [n, K] (K a multiple
-// of 16) into dst [n][row_bytes], zeros up to a multiple of 128, and their scales, here and in
-// the cluster's other CTAs. C: 256-value pieces of a row that the warp keeps in registers
-// (0: a longer row, read twice).
-template <typename T, int R, int C>
-__device__ __forceinline__ void quant_rows(const T* __restrict__ src, int n, int K, int i0, int step, uint8_t* dst,
-                                           int row_bytes, float* scale, int lane, int peers) {
+// int8 rows of src [n, K] (K a multiple of 16) into dst [n][row_bytes], zeros up to a multiple
+// of 128, and their scales, here and in the cluster's other CTAs: this CTA's part are rows
+// rank, rank + peers, ... The last `threads` threads of the CTA take part, eight values each
+// at a time; they meet at named barrier 1. top: [n] scratch.
+template <typename T>
+__device__ void quant_rows(const T* __restrict__ src, int n, int K, int rank, int peers, int threads, uint8_t* dst,
+                           int row_bytes, float* scale, uint32_t* top) {
   const int nc = K >> 3, padded = (K + 127) / 128 * 16;
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  const uint4* s[R];
-  uint4 raw[R][C > 0 ? C : 1];
-  float amax[R], inv[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    s[r] = reinterpret_cast<const uint4*>(src + static_cast<int64_t>(min(i0 + r * step, n - 1)) * K);
-    amax[r] = 0.0f;
-#pragma unroll
-    for (int c = 0; c < C; ++c) raw[r][c] = lane + c * 32 < nc ? s[r][lane + c * 32] : zero;
-  }
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    if constexpr (C > 0) {
-#pragma unroll
-      for (int c = 0; c < C; ++c) amax[r] = fmaxf(amax[r], abs_max8<T>(raw[r][c]));
-    } else {
-#pragma unroll 8
-      for (int c = lane; c < nc; c += 32) amax[r] = fmaxf(amax[r], abs_max8<T>(s[r][c]));
+  const int t0 = static_cast<int>(threadIdx.x) - (kThreads - threads);
+  if (t0 < 0) return;
+  for (int i = rank + t0 * peers; i < n; i += threads * peers) top[i] = 0u;
+  named_bar_sync(1, threads);
+  const uint4* rows = reinterpret_cast<const uint4*>(src);
+  // Piece c of row i: this thread's pieces in turn, `per` to a row (zeros behind K), with the
+  // loads of the next four in flight. (A queue, not an unrolled loop: short code.)
+  struct Pos {
+    int i, c;
+  };
+  auto settle = [&](Pos& p, int per) {
+    while (p.c >= per) {
+      p.c -= per;
+      p.i += peers;
     }
-    amax[r] = moe::warp_max(amax[r]);
-    inv[r] = quant_inv(amax[r]);
-    const int i = i0 + r * step;
-    if (lane == 0 && i < n) share(scale + i, quant_scale(amax[r]), peers);
-  }
-  auto put = [&](int r, int c, const uint4& u) {
+  };
+  auto each = [&](int per, auto&& f) {
+    Pos at{rank, t0}, ahead{rank, t0};
+    auto fetch = [&]() {
+      settle(ahead, per);
+      uint4 u = make_uint4(0u, 0u, 0u, 0u);
+      if (ahead.i < n && ahead.c < nc) u = rows[static_cast<int64_t>(ahead.i) * nc + ahead.c];
+      ahead.c += threads;
+      return u;
+    };
+    uint4 q0 = fetch(), q1 = fetch(), q2 = fetch(), q3 = fetch();
+#pragma unroll 1
+    for (settle(at, per); at.i < n; settle(at, per)) {
+      const uint4 u = q0;
+      q0 = q1;
+      q1 = q2;
+      q2 = q3;
+      q3 = fetch();
+      f(at.i, at.c, u);
+      at.c += threads;
+    }
+  };
+  each(nc, [&](int i, int, const uint4& u) {
+    // (a NaN is no maximum)
+    atomicMax(&top[i], __float_as_uint(fmaxf(abs_max8<T>(u), 0.0f)));
+  });
+  named_bar_sync(1, threads);
+  each(padded, [&](int i, int c, const uint4& u) {
+    const float amax = __uint_as_float(top[i]), inv = quant_inv(amax);
     float f[8];
     unpack8<T>(u, f);
-    uint2 w = make_uint2(quant4(f, inv[r]), quant4(f + 4, inv[r]));
+    uint2 w = make_uint2(quant4(f, inv), quant4(f + 4, inv));
     if (c >= nc) w = make_uint2(0u, 0u);  // (an infinite or NaN factor makes no zero of a zero)
-    const int i = i0 + r * step;
-    if (i < n && c < padded) share(reinterpret_cast<uint2*>(dst + i * row_bytes + c * 8), w, peers);
-  };
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    if constexpr (C > 0) {
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-        if (c * 32 < padded) put(r, lane + c * 32, raw[r][c]);
-    } else {
-#pragma unroll 4
-      for (int c = lane; c < padded; c += 32) put(r, c, c < nc ? s[r][c] : zero);
-    }
-  }
-}
-
-// All rows of src [n, K], dealt out to the warps of the cluster's CTAs, R at a time.
-template <typename T, int R>
-__device__ __forceinline__ void quant_all(const T* __restrict__ src, int n, int K, int worker, int workers, uint8_t* dst,
-                                          int row_bytes, float* scale, int lane, int peers) {
-  if (K <= 1024) {
-    for (int i = worker; i < n; i += R * workers)
-      quant_rows<T, R, 4>(src, n, K, i, workers, dst, row_bytes, scale, lane, peers);
-  } else if (K <= 2048) {
-    for (int i = worker; i < n; i += workers)
-      quant_rows<T, 1, 8>(src, n, K, i, workers, dst, row_bytes, scale, lane, peers);
-  } else {
-    for (int i = worker; i < n; i += workers)
-      quant_rows<T, 1, 0>(src, n, K, i, workers, dst, row_bytes, scale, lane, peers);
-  }
+    share(reinterpret_cast<uint2*>(dst + i * row_bytes + c * 8), w, peers);
+    if (c == 0) share(scale + i, quant_scale(amax), peers);
+  });
 }
 
 __device__ __forceinline__ void route_one(const Layer& p, int t, int lane, int* slot_e, float* slot_w, int peers) {
@@ -261,68 +258,56 @@ __device__ __forceinline__ void route_one(const Layer& p, int t, int lane, int* 
 }
 
 // Entries: the slots of each expert, at most kEntry to an entry (an id that appears more often
-// has several), slots in order. A slot whose id is outside [0, E) is in none. masks: for each
-// expert the slots that name it, a bit each. Returns the number of entries; every thread of
-// the CTA takes part.
+// has several), by expert, slots in order. A slot whose id is outside [0, E) is in none. masks:
+// zeroed, for each expert the slots that name it, a bit each. Returns the number of entries;
+// every thread of the CTA takes part.
 __device__ int list_entries(const int* slot_e, int n, int E, int* ent_e, int* ent_n, uint16_t* list, uint32_t* masks) {
-  __shared__ int warp_sum[2 * kWarps];
-  __shared__ int16_t ent_of[kMaxSlots];  // of an entry's first slot
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int words = (n + 31) >> 5;
-  for (int i = threadIdx.x; i < E * words; i += kThreads) masks[i] = 0u;
-  __syncthreads();
+  __shared__ int total;
+  __shared__ int16_t first[kMaxExperts];  // entry of an expert's first slots
+  const int lane = threadIdx.x & 31, words = (n + 31) >> 5;
+#pragma unroll 1
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const int e = slot_e[i];
     if (e >= 0 && e < E) atomicOr(&masks[e * words + (i >> 5)], 1u << (i & 31));
   }
   __syncthreads();
-  static_assert(kMaxSlots <= 2 * kThreads, "two slots to a thread");
-  int total = 0, rank[2] = {-1, -1};
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    if (r * kThreads < n) {
-      const int i = r * kThreads + threadIdx.x;
-      const int e = i < n ? slot_e[i] : -1;
-      int before = -1, all = 0;
-      if (e >= 0 && e < E) {
-        before = 0;
-        for (int w = 0; w < words; ++w) {
-          const uint32_t m = masks[e * words + w];
-          const int bit = i - w * 32;
-          before += __popc(bit >= 32 ? m : bit <= 0 ? 0u : m & ((1u << bit) - 1u));
-          all += __popc(m);
-        }
+  if (threadIdx.x < 32) {
+    int at = 0;
+#pragma unroll 1
+    for (int e0 = 0; e0 < E; e0 += 32) {
+      const int e = e0 + lane;
+      int c = 0;
+      if (e < E) {
+#pragma unroll 1
+        for (int w = 0; w < words; ++w) c += __popc(masks[e * words + w]);
       }
-      rank[r] = before;
-      const bool opens = before >= 0 && before % kEntry == 0;
-      const unsigned m = __ballot_sync(0xffffffffu, opens);
-      if (lane == 0) warp_sum[r * kWarps + warp] = __popc(m);
-      __syncthreads();
-      int at = total;
-      for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) at += warp_sum[r * kWarps + w];
-        total += warp_sum[r * kWarps + w];
+      const int ne = (c + kEntry - 1) / kEntry;
+      int sum = ne;
+#pragma unroll 1
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
       }
-      if (opens) {
-        const int a = at + __popc(m & ((1u << lane) - 1u));
-        ent_of[i] = static_cast<int16_t>(a);
-        ent_e[a] = e;
-        ent_n[a] = min(kEntry, all - before);
+      const int a = at + sum - ne;
+      if (ne > 0) first[e] = static_cast<int16_t>(a);
+#pragma unroll 1
+      for (int j = 0; j < ne; ++j) {
+        ent_e[a + j] = e;
+        ent_n[a + j] = min(kEntry, c - j * kEntry);
       }
+      at += __shfl_sync(0xffffffffu, sum, 31);
     }
+    if (lane == 0) total = at;
   }
   __syncthreads();
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    if (rank[r] >= 0) {
-      // the entry's first slot: the one of rank [rank / kEntry] * kEntry
-      const int i = r * kThreads + threadIdx.x;
-      const uint32_t* mk = masks + slot_e[i] * words;
-      int left = rank[r] / kEntry * kEntry, w = 0;
-      while (left >= __popc(mk[w])) left -= __popc(mk[w++]);
-      uint32_t bits = mk[w];
-      for (; left > 0; --left) bits &= bits - 1u;
-      list[ent_of[w * 32 + __ffs(bits) - 1] * kEntry + rank[r] % kEntry] = static_cast<uint16_t>(i);
+#pragma unroll 1
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const int e = slot_e[i];
+    if (e >= 0 && e < E) {
+      int before = __popc(masks[e * words + (i >> 5)] & ((1u << (i & 31)) - 1u));
+#pragma unroll 1
+      for (int w = 0; w < i >> 5; ++w) before += __popc(masks[e * words + w]);
+      list[(first[e] + before / kEntry) * kEntry + before % kEntry] = static_cast<uint16_t>(i);
     }
   }
   __syncthreads();
@@ -334,7 +319,7 @@ __device__ int list_entries(const int* slot_e, int n, int E, int* ent_e, int* en
 template <int NT>
 __device__ __forceinline__ void stage_product(int (&acc)[NT][4], const uint8_t* st, int g, int q,
                                               const uint8_t* const (&x)[NT], int k0, int K) {
-#pragma unroll
+#pragma unroll 1
   for (int c = 0; c < 2; ++c) {
     if (k0 + c * 128 >= K) break;
 #pragma unroll
@@ -374,18 +359,21 @@ __global__ void __launch_bounds__(kThreads) few_gate_up(const __grid_constant__ 
     for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1);
     fence_barrier_init();
   }
+  for (int i = threadIdx.x; i < p.E * ((n + 31) >> 5); i += kThreads) reinterpret_cast<uint32_t*>(smem + pl.masks)[i] = 0u;
   const int rank = static_cast<int>(cluster_ctarank()), peers = static_cast<int>(cluster_nctarank());
-  const int workers = peers * kWarps;
   if (peers > 1) cluster_sync_all();  // the peers have started
   pdl_wait();
-  // routing on the first warps of every CTA, the rows on the last, so that both run at once
+  // the first warps route this CTA's tokens, the others quantise its rows meanwhile
+  int routers = 0;
   if (p.logits != nullptr) {
-    for (int t = warp * peers + rank; t < p.T; t += workers) route_one(p, t, lane, slot_e, slot_w, peers);
+    routers = min(kWarps / 2, (p.T - rank + peers - 1) / peers);
+    if (warp < routers)
+      for (int t = warp * peers + rank; t < p.T; t += routers * peers) route_one(p, t, lane, slot_e, slot_w, peers);
   } else {
     for (int i = threadIdx.x; i < n; i += kThreads) slot_e[i] = p.topi[i];
   }
-  quant_all<T, 1>(static_cast<const T*>(p.x), p.T, p.H, (kWarps - 1 - warp) * peers + rank, workers, codes, pl.row, a_s,
-                  lane, peers);
+  quant_rows<T>(static_cast<const T*>(p.x), p.T, p.H, rank, peers, 32 * (kWarps - routers), codes, pl.row, a_s,
+                reinterpret_cast<uint32_t*>(smem + pl.top));
   join(peers);
   const int n_ent = list_entries(slot_e, n, p.E, ent_e, ent_n, list, reinterpret_cast<uint32_t*>(smem + pl.masks));
 
@@ -481,19 +469,23 @@ __global__ void __launch_bounds__(kThreads) few_gate_up(const __grid_constant__ 
     if (cnt <= 8) run(std::integral_constant<int, 1>{});
     else run(std::integral_constant<int, 2>{});
     if (!ok) break;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int at = i * 8 + 2 * q + r;
-        if (at < cnt) {
-          const int slot = list[a * kEntry + at];
-          const float as = a_s[slot / p.k];
-          const float gate = round_trip<T>(__fmul_rn(__fmul_rn(__int2float_rn(acc[i][r]), as), sg));
-          const float up = round_trip<T>(__fmul_rn(__fmul_rn(__int2float_rn(acc[i][2 + r]), as), su));
-          static_cast<T*>(p.h)[static_cast<int64_t>(slot) * p.I + c * 8 + g] = act_mul_one<T, ACT>(gate, up);
-        }
+    // column c * 8 + g of this lane's slots 2 q, 2 q + 1 (and 8 + those)
+#pragma unroll 1
+    for (int j = 0; j < 4; ++j) {
+      const int at = (j >> 1) * 8 + 2 * q + (j & 1);
+      if (at < cnt) {
+        const int slot = list[a * kEntry + at];
+        const float as = a_s[slot / p.k];
+        const float gate = round_trip<T>(__fmul_rn(__fmul_rn(__int2float_rn(acc[0][0]), as), sg));
+        const float up = round_trip<T>(__fmul_rn(__fmul_rn(__int2float_rn(acc[0][2]), as), su));
+        static_cast<T*>(p.h)[static_cast<int64_t>(slot) * p.I + c * 8 + g] = act_mul_one<T, ACT>(gate, up);
       }
+      if (j == 1 && cnt <= 8) break;
+      const bool odd = (j & 1) != 0;  // the next slot's accumulators to the front
+      acc[0][0] = odd ? acc[1][0] : acc[0][1];
+      acc[0][2] = odd ? acc[1][2] : acc[0][3];
+      acc[0][1] = acc[1][1];
+      acc[0][3] = acc[1][3];
     }
   }
   // after a wait that gave up: the loads still in flight land before the CTA leaves
@@ -529,14 +521,14 @@ __global__ void __launch_bounds__(kThreads) few_down(const __grid_constant__ CUt
     fence_barrier_init();
   }
   const int rank = static_cast<int>(cluster_ctarank()), peers = static_cast<int>(cluster_nctarank());
-  const int workers = peers * kWarps;
   if (peers > 1) cluster_sync_all();  // the peers have started
   int n_ent;
   if (p.early) {
+    for (int i = threadIdx.x; i < p.E * ((n + 31) >> 5); i += kThreads) reinterpret_cast<uint32_t*>(smem + pl.masks)[i] = 0u;
     // The routing's inputs are older than few_gate_up, which released this kernel after its own
     // wait for them: they are read before this kernel waits for few_gate_up.
     if (p.logits != nullptr) {
-      for (int t = warp * peers + rank; t < p.T; t += workers) route_one(p, t, lane, slot_e, slot_w, peers);
+      for (int t = warp * peers + rank; t < p.T; t += kWarps * peers) route_one(p, t, lane, slot_e, slot_w, peers);
     } else {
       for (int i = threadIdx.x; i < n; i += kThreads) {
         slot_e[i] = p.topi[i];
@@ -588,7 +580,8 @@ __global__ void __launch_bounds__(kThreads) few_down(const __grid_constant__ CUt
   if (lane == 0)
     for (int i = 0; i < issued; ++i) issue();
   pdl_wait();
-  quant_all<T, 2>(static_cast<const T*>(p.h), n, p.I, warp * peers + rank, workers, codes, pl.row, h_s, lane, peers);
+  quant_rows<T>(static_cast<const T*>(p.h), n, p.I, rank, peers, kThreads, codes, pl.row, h_s,
+                reinterpret_cast<uint32_t*>(smem + pl.top));
   join(peers);
   pdl_launch_dependents();
 
@@ -686,7 +679,7 @@ int few_status_read_and_clear(int* code) {
 namespace {
 
 #ifndef FEW_MIN
-#define FEW_MIN 24
+#define FEW_MIN 16384
 #endif
 constexpr int kSmemMax = 226 * 1024;  // static shared memory (the entry list's) beside it
 
@@ -698,7 +691,7 @@ int few_stages(int rows, int64_t k_len, int slots, int E, int extra) {
 }
 
 // CTAs per cluster that share the preparation: with few rows it costs more than it saves.
-int few_cluster(int64_t rows) { return rows >= FEW_MIN ? 8 : 1; }
+int few_cluster(int64_t rows, int64_t k_len) { return rows * k_len >= FEW_MIN ? 8 : 1; }
 
 // Grid of `want` CTAs at most, in clusters of cs that are resident at once.
 int few_grid(int64_t want, int smem, int cs) {
@@ -762,7 +755,7 @@ template <typename T, int ACT, bool WIDE_GU>
 int launch_gate_up(const few::Layer& p, const CUtensorMap& map, int smem, cudaStream_t st) {
   static std::atomic<bool> done[kMaxDevices] = {};
   if (int s = configure(few::few_gate_up<T, ACT, WIDE_GU>, done)) return s;
-  const int cs = few_cluster(p.T * p.k);
+  const int cs = few_cluster(p.T, p.H);
   // units at most: every slot its own expert
   const int grid = few_grid((int64_t)p.T * p.k * (p.I / 8), smem, cs);
   launch_cluster(few::few_gate_up<T, ACT, WIDE_GU>, grid, cs, smem, st, map, p);
@@ -773,7 +766,7 @@ template <typename T, bool WIDE_DN>
 int launch_down(const few::Layer& p, const CUtensorMap& map, int smem, cudaStream_t st) {
   static std::atomic<bool> done[kMaxDevices] = {};
   if (int s = configure(few::few_down<T, WIDE_DN>, done)) return s;
-  const int cs = few_cluster(p.T * p.k);
+  const int cs = few_cluster(p.T * p.k, p.I);
   launch_cluster(few::few_down<T, WIDE_DN>, few_grid(p.H / 16, smem, cs), cs, smem, st, map, p);
   return FNI8_OK;
 }
@@ -803,7 +796,7 @@ int launch_few(const few::Layer& layer, int act, const CUtensorMap& gu, const CU
 }  // namespace
 
 bool few_supported(int64_t T, int64_t H, int64_t k, int64_t E, int64_t I) {
-  if (T < 1 || T > few::kMaxTokens || k < 1 || k > 32 || T * k > few::kMaxSlots || E < 1 || E > 512) return false;
+  if (T < 1 || T > few::kMaxTokens || k < 1 || k > 32 || T * k > few::kMaxSlots || E < 1 || E > few::kMaxExperts) return false;
   if (H % 16 != 0 || I % 16 != 0 || H > (1 << 17) || I > (1 << 17)) return false;
   const int n = (int)(T * k);
   return few_stages((int)T, H, n, (int)E, 0) > 0 && few_stages(n, I, n, (int)E, n * 64) > 0;

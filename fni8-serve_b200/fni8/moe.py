@@ -30,7 +30,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _native as nat
-from .ops import _ACT, _DT, _need_cuda, _stream, _vp, act_and_mul, linear
+from .ops import _ACT, _DT, _launch, _need_cuda, _ptr, _stream, _vp, act_and_mul, linear
 from .qtensor import QTensor
 
 
@@ -205,7 +205,8 @@ def layer(x: torch.Tensor, logits: torch.Tensor, stack: ExpertStack, top_k: int,
     dev = x.device
     if logits.device != dev or stack.w_gu.device != dev:
         raise RuntimeError("fni8.moe.layer: x, logits and experts are on different devices")
-    x2, lg = x.contiguous(), logits.float().contiguous()
+    x2 = x.contiguous()
+    lg = (logits if logits.dtype == torch.float32 else logits.float()).contiguous()
     T, H = x2.shape
     bias = None
     if sel_bias is not None and scoring == "sigmoid":
@@ -216,11 +217,10 @@ def layer(x: torch.Tensor, logits: torch.Tensor, stack: ExpertStack, top_k: int,
     wsb = nat.lib().fni8_moe_layer_workspace_bytes(T, H, top_k, E, I)
     ws = torch.empty(max(wsb, 1), dtype=torch.uint8, device=dev)
     out = torch.empty_like(x2)
-    with torch.cuda.device(dev):
-        nat.call("fni8_moe_layer_w8a8", _vp(x2), _DT[x.dtype], T, H, _vp(lg), top_k,
-                 nat.SCORE_SOFTMAX if scoring == "softmax" else nat.SCORE_SIGMOID, _vp(bias), ng,
-                 int(topk_group) if ng else 0, int(norm_topk_prob), scaling, _vp(stack.w_gu), _vp(stack.s_gu),
-                 _vp(stack.w_dn), _vp(stack.s_dn), E, I, _ACT[act], _vp(out), _vp(ws), wsb, _stream(dev))
+    _launch("fni8_moe_layer_w8a8", dev, x2.data_ptr(), _DT[x.dtype], T, H, lg.data_ptr(), top_k,
+            nat.SCORE_SOFTMAX if scoring == "softmax" else nat.SCORE_SIGMOID, _ptr(bias), ng, int(topk_group) if ng else 0,
+            int(norm_topk_prob), scaling, stack.w_gu.data_ptr(), stack.s_gu.data_ptr(), stack.w_dn.data_ptr(),
+            stack.s_dn.data_ptr(), E, I, _ACT[act], out.data_ptr(), ws.data_ptr(), wsb)
     return out
 
 

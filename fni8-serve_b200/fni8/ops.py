@@ -46,6 +46,34 @@ def _stream(dev: torch.device):
     return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
 
 
+def _ptr(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+# the current stream's handle without building a Stream object (2 us of a small op's call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _launch(name: str, dev: torch.device, *args) -> None:
+    """Call entry point `name` on dev's current stream, with dev as the current device."""
+    index = dev.index
+    if index == torch.cuda.current_device():
+        status = getattr(nat.lib(), name)(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = getattr(nat.lib(), name)(*args, _raw_stream(index))
+    if status:
+        nat.check(status, name)
+
+
+def _rows(x: torch.Tensor, K: int) -> torch.Tensor:
+    """x[..., K] as contiguous rows [M, K]."""
+    if x.dim() != 2:
+        x = x.reshape(-1, K)
+    return x if x.is_contiguous() else x.contiguous()
+
+
 def _need_cuda(x: torch.Tensor, what: str) -> None:
     if not x.is_cuda:
         raise RuntimeError(f"fni8.{what}: expected a CUDA tensor (fni8-serve_b200 has no CPU path)")
@@ -415,15 +443,16 @@ def quantize_fp4(x: torch.Tensor, scheme: str = "mxfp4") -> QTensor:
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError("fni8.quantize_fp4: empty rows")
     K, lead, dev = x.shape[-1], x.shape[:-1], x.device
-    x2 = x.reshape(-1, K).contiguous()
+    x2 = _rows(x, K)
     M = x2.shape[0]
     q = torch.empty((M, (K + 31) // 32 * 16), dtype=torch.uint8, device=dev)
     sf = torch.empty(((M + 127) // 128, (K + 4 * g - 1) // (4 * g), 512), dtype=torch.uint8, device=dev)
     rs = torch.empty((M,), dtype=torch.float32, device=dev) if scheme == "nvfp4" else None
-    with torch.cuda.device(dev):
-        nat.call("fni8_quantize_rows_fp4", _vp(x2), dt, fmt, M, K, _vp(q), _vp(sf), _vp(rs), _stream(dev))
-    return QTensor(q.reshape(*lead, q.shape[1]) if x.dim() != 2 else q, sf, scheme=scheme, group_size=g,
-                   row_scale=rs if rs is None or x.dim() == 2 else rs.reshape(lead), cols=K)
+    _launch("fni8_quantize_rows_fp4", dev, x2.data_ptr(), dt, fmt, M, K, q.data_ptr(), sf.data_ptr(), _ptr(rs))
+    if x.dim() != 2:
+        q = q.reshape(*lead, q.shape[1])
+        rs = None if rs is None else rs.reshape(lead)
+    return QTensor(q, sf, scheme=scheme, group_size=g, row_scale=rs, cols=K)
 
 
 def dequantize_fp4(qt: QTensor, dtype: torch.dtype = torch.float16) -> torch.Tensor:
@@ -436,9 +465,8 @@ def dequantize_fp4(qt: QTensor, dtype: torch.dtype = torch.float16) -> torch.Ten
         raise TypeError(f"fni8.dequantize_fp4: dtype must be float16, bfloat16 or float32, got {dtype}")
     dev = qt.data.device
     out = torch.empty((*qt.data.shape[:-1], K), dtype=dtype, device=dev)
-    with torch.cuda.device(dev):
-        nat.call("fni8_dequantize_rows_fp4", _vp(qt.data), _vp(qt.scale), _vp(qt.row_scale), _FP4[qt.scheme][0], M, K,
-                 _vp(out), odt, _stream(dev))
+    _launch("fni8_dequantize_rows_fp4", dev, qt.data.data_ptr(), qt.scale.data_ptr(), _ptr(qt.row_scale),
+            _FP4[qt.scheme][0], M, K, out.data_ptr(), odt)
     return out
 
 
@@ -475,9 +503,8 @@ def linear_fp4(xq: QTensor, qt: QTensor, bias: torch.Tensor | None = None,
     N = _fp4_weight(qt, K, dev, "linear_fp4")
     b = _fp4_bias(bias, N, out_dtype, dev, "linear_fp4")
     out = torch.empty((*xq.data.shape[:-1], N), dtype=out_dtype, device=dev)
-    with torch.cuda.device(dev):
-        nat.call("fni8_gemm_fp4", _vp(xq.data), _vp(xq.scale), _vp(xq.row_scale), _vp(qt.data), _vp(qt.scale),
-                 _vp(qt.row_scale), _vp(b), _vp(out), _DT[out_dtype], _FP4[qt.scheme][0], M, N, K, _stream(dev))
+    _launch("fni8_gemm_fp4", dev, xq.data.data_ptr(), xq.scale.data_ptr(), _ptr(xq.row_scale), qt.data.data_ptr(),
+            qt.scale.data_ptr(), _ptr(qt.row_scale), _ptr(b), out.data_ptr(), _DT[out_dtype], _FP4[qt.scheme][0], M, N, K)
     return out
 
 
@@ -487,17 +514,22 @@ def _linear_fp4(x: torch.Tensor, qt: QTensor, bias: torch.Tensor | None) -> torc
     fmt, g = _FP4[qt.scheme]
     K, dev = x.shape[-1], x.device
     N = _fp4_weight(qt, K, dev, "linear")
-    x2 = x.reshape(-1, K).contiguous()
+    x2 = _rows(x, K)
     M = x2.shape[0]
     b = _fp4_bias(bias, N, x.dtype, dev, "linear")
     out = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev)
-    sb = nat.lib().fni8_linear_fp4_scratch_bytes(fmt, M, N, K)  # 0: one kernel that quantises x itself
-    if sb == 0 and x2.data_ptr() & 15:
-        x2 = x2.clone()
-    scratch = torch.empty(sb, dtype=torch.uint8, device=dev) if sb else None
-    with torch.cuda.device(dev):
-        nat.call("fni8_linear_fp4", _vp(x2), dt, _vp(qt.data), _vp(qt.scale), _vp(qt.row_scale), _vp(b), _vp(out), fmt,
-                 M, N, K, _vp(scratch), sb, _stream(dev))
+    scratch, sb = None, 0
+    if M > 16 or K % 8:
+        # scale tiles, codes, row scales
+        sb = (M + 127) // 128 * ((K + 4 * g - 1) // (4 * g)) * 512 + M * ((K + 31) // 32 * 16 + 4)
+    else:
+        sb = nat.lib().fni8_linear_fp4_scratch_bytes(fmt, M, N, K)  # 0: one kernel that quantises x itself
+        if sb == 0 and x2.data_ptr() & 15:
+            x2 = x2.clone()
+    if sb:
+        scratch = torch.empty(sb, dtype=torch.uint8, device=dev)
+    _launch("fni8_linear_fp4", dev, x2.data_ptr(), dt, qt.data.data_ptr(), qt.scale.data_ptr(), _ptr(qt.row_scale),
+            _ptr(b), out.data_ptr(), fmt, M, N, K, _ptr(scratch), sb)
     return out
 
 
