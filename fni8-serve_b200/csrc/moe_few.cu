@@ -15,16 +15,17 @@
 // At one MMA for 512 weight bytes the SM's share of HBM asks for one in 22 cycles.
 //
 //  * Every warp is on its own: it takes (expert, 16 weight rows) units, and lane 0 streams
-//    them through the warp's private ring of 4 KB stages by TMA (16 rows x 256 bytes,
+//    them through the warp's private ring of stages by TMA (16 rows x 256 or 512 bytes,
 //    128-byte swizzle). There is no producer warp and no barrier between warps.
 //  * In few_gate_up the 16 rows are 8 gate rows and the 8 matching up rows: an accumulator
 //    fragment holds gate and up of the same column and slot in one lane, so act(g) * u needs
 //    no exchange. In few_down a CTA owns 16 output columns through all experts, keeps their
-//    y in shared memory and sums each token's k slots there: no atomics, no third kernel.
-//  * Each CTA routes, quantises the rows and lists the experts for itself (T rows of x, the
-//    T k rows of h): cheaper than a launch that would hand them over. Where both kernels fit
-//    on an SM few_down does that too, and starts its weight loads, before it waits for
-//    few_gate_up; where they do not it reads the lists that few_gate_up leaves.
+//    int32 sums in shared memory and joins each token's k slots there: no atomics in global
+//    memory, no third kernel. With fewer experts than warps it splits their K.
+//  * Each CTA, or each cluster of eight where there are many values, routes, quantises the
+//    rows and lists the experts for itself: cheaper than a launch that would hand them over.
+//    Where both kernels fit on an SM few_down does that too, and starts its weight loads, before
+//    it waits for few_gate_up; where they do not it reads the lists that few_gate_up leaves.
 //  * A CTA runs most of its code once, and an instruction line that is not in its SM's caches
 //    costs 0.1 us and more; so the preparation is short loops, not unrolled ones (listing the
 //    experts of one token: 4.9 us at first sight, 0.8 us the second time), and the weights pass
@@ -44,7 +45,9 @@ namespace few {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kStage = 4096;  // 16 weight rows x 256 bytes
+// A stage: 16 weight rows x 2 or 4 128-byte columns of K. Four stream faster (512 contiguous
+// bytes of a row; 4 tokens through large experts 74 -> 65 us), two let both kernels share an SM.
+__host__ __device__ constexpr int stage_bytes(int cols) { return 16 * 128 * cols; }
 constexpr int kEntry = 16;    // slots of one expert in one entry (two n8 tiles)
 constexpr int kMaxTokens = 16;
 constexpr int kMaxSlots = 512;
@@ -83,9 +86,9 @@ struct Layer {
 struct Plan {
   int row, codes, slot_e, slot_w, scale, top, ent_e, ent_n, list, masks, extra, bars, total;
 };
-__host__ __device__ inline Plan make_plan(int stages, int rows, int k_len, int slots, int E, int extra_bytes) {
+__host__ __device__ inline Plan make_plan(int cols, int stages, int rows, int k_len, int slots, int E, int extra_bytes) {
   Plan p;
-  int o = kWarps * stages * kStage;
+  int o = kWarps * stages * stage_bytes(cols);
   auto take = [&](int bytes) {
     const int at = o;
     o += (bytes + 15) & ~15;
@@ -314,13 +317,13 @@ __device__ int list_entries(const int* slot_e, int n, int E, int* ent_e, int* en
   return total;
 }
 
-// One stage (16 weight rows x 256 bytes from k0 on, in two 128-byte columns; none behind K)
+// One stage (16 weight rows x COLS 128-byte columns from k0 on; none behind K)
 // times up to 8 NT slots, whose code rows lane (g, q) reads at x[.].
-template <int NT>
+template <int NT, int COLS>
 __device__ __forceinline__ void stage_product(int (&acc)[NT][4], const uint8_t* st, int g, int q,
                                               const uint8_t* const (&x)[NT], int k0, int K) {
 #pragma unroll 1
-  for (int c = 0; c < 2; ++c) {
+  for (int c = 0; c < COLS; ++c) {
     if (k0 + c * 128 >= K) break;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -338,12 +341,13 @@ __device__ __forceinline__ void stage_product(int (&acc)[NT][4], const uint8_t* 
   }
 }
 
-template <typename T, int ACT, bool WIDE>
+template <typename T, int ACT, bool WIDE, int COLS>
 __global__ void __launch_bounds__(kThreads) few_gate_up(const __grid_constant__ CUtensorMap tmW, Layer p) {
+  constexpr int kStageK = 128 * COLS, kStage = stage_bytes(COLS);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int n = p.T * p.k;
-  const Plan pl = make_plan(p.stages, p.T, p.H, n, p.E, 0);
+  const Plan pl = make_plan(COLS, p.stages, p.T, p.H, n, p.E, 0);
   uint8_t* codes = smem + pl.codes;
   int* slot_e = reinterpret_cast<int*>(smem + pl.slot_e);
   float* slot_w = reinterpret_cast<float*>(smem + pl.slot_w);
@@ -390,7 +394,7 @@ __global__ void __launch_bounds__(kThreads) few_gate_up(const __grid_constant__ 
   }
   pdl_launch_dependents();
 
-  const int U = p.I >> 3, KC = (p.H + 255) >> 8;
+  const int U = p.I >> 3, KC = (p.H + kStageK - 1) / kStageK;
   const int first = warp * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x);
   const int stride = kWarps * static_cast<int>(gridDim.x);
   const int total = n_ent * U;
@@ -405,13 +409,13 @@ __global__ void __launch_bounds__(kThreads) few_gate_up(const __grid_constant__ 
     uint64_t* bar = &full[ps];
     const int e = ent_e[pa], c = pc * 8;
     mbar_arrive_expect_tx(bar, kStage);
-    if constexpr (WIDE) {  // 128 bytes x 8 rows x {gate, up} x 2 columns
-      tma_load_5d(&tmW, bar, dst, 0, c, 0, pk * 2, e, policy);
+    if constexpr (WIDE) {  // 128 bytes x 8 rows x {gate, up} x COLS columns
+      tma_load_5d(&tmW, bar, dst, 0, c, 0, pk * COLS, e, policy);
     } else {
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        tma_load_3d(&tmW, bar, dst + hh * 2048, pk * 256 + hh * 128, c, e, policy);
-        tma_load_3d(&tmW, bar, dst + hh * 2048 + 1024, pk * 256 + hh * 128, p.I + c, e, policy);
+      for (int hh = 0; hh < COLS; ++hh) {
+        tma_load_3d(&tmW, bar, dst + hh * 2048, pk * kStageK + hh * 128, c, e, policy);
+        tma_load_3d(&tmW, bar, dst + hh * 2048 + 1024, pk * kStageK + hh * 128, p.I + c, e, policy);
       }
     }
     if (++pk == KC) {
@@ -451,7 +455,7 @@ __global__ void __launch_bounds__(kThreads) few_gate_up(const __grid_constant__ 
         ok = mbar_wait(&full[s], ph, &g_status, kCodeGateUp);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        stage_product<NT>(part, ring + s * kStage, g, q, x, kc * 256, p.H);
+        stage_product<NT, COLS>(part, ring + s * kStage, g, q, x, kc * kStageK, p.H);
         ++consumed;
         __syncwarp();
         if (lane == 0 && issued < steps) issue();
@@ -498,12 +502,13 @@ __global__ void __launch_bounds__(kThreads) few_gate_up(const __grid_constant__ 
   }
 }
 
-template <typename T, bool WIDE>
+template <typename T, bool WIDE, int COLS>
 __global__ void __launch_bounds__(kThreads) few_down(const __grid_constant__ CUtensorMap tmW, Layer p) {
+  constexpr int kStageK = 128 * COLS, kStage = stage_bytes(COLS);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int n = p.T * p.k;
-  const Plan pl = make_plan(p.stages, n, p.I, n, p.E, n * 64);
+  const Plan pl = make_plan(COLS, p.stages, n, p.I, n, p.E, n * 64);
   uint8_t* codes = smem + pl.codes;
   int* slot_e = reinterpret_cast<int*>(smem + pl.slot_e);
   float* slot_w = reinterpret_cast<float*>(smem + pl.slot_w);
@@ -511,7 +516,7 @@ __global__ void __launch_bounds__(kThreads) few_down(const __grid_constant__ CUt
   int* ent_e = reinterpret_cast<int*>(smem + pl.ent_e);
   int* ent_n = reinterpret_cast<int*>(smem + pl.ent_n);
   uint16_t* list = reinterpret_cast<uint16_t*>(smem + pl.list);
-  float* y = reinterpret_cast<float*>(smem + pl.extra);  // [slots][16]
+  int* y = reinterpret_cast<int*>(smem + pl.extra);  // [slots][16] sums of the tile
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + pl.bars) + warp * 4;
   uint8_t* ring = smem + warp * p.stages * kStage;
@@ -522,6 +527,7 @@ __global__ void __launch_bounds__(kThreads) few_down(const __grid_constant__ CUt
   }
   const int rank = static_cast<int>(cluster_ctarank()), peers = static_cast<int>(cluster_nctarank());
   if (peers > 1) cluster_sync_all();  // the peers have started
+  for (int i = threadIdx.x; i < n * 16; i += kThreads) y[i] = 0;
   int n_ent;
   if (p.early) {
     for (int i = threadIdx.x; i < p.E * ((n + 31) >> 5); i += kThreads) reinterpret_cast<uint32_t*>(smem + pl.masks)[i] = 0u;
@@ -551,31 +557,45 @@ __global__ void __launch_bounds__(kThreads) few_down(const __grid_constant__ CUt
     __syncthreads();
   }
 
-  const int KC = (p.I + 255) >> 8, tiles = p.H >> 4;
+  const int KC = (p.I + kStageK - 1) / kStageK, tiles = p.H >> 4;
   const int my_tiles = (tiles - static_cast<int>(blockIdx.x) - 1 + static_cast<int>(gridDim.x)) / static_cast<int>(gridDim.x);
-  const int my_ents = n_ent > warp ? (n_ent - warp - 1) / kWarps + 1 : 0;
-  const int steps = my_tiles * my_ents * KC;
-  int pt = static_cast<int>(blockIdx.x), pa = warp, pk = 0, ps = 0;
+  // Fewer entries than warps: an entry's K range is cut into 2^lg parts, so that no warp idles
+  // (one token through 2 experts of 4096 x 4096: 40 -> 32 us).
+  int lg = 0;
+  while (n_ent << (lg + 1) <= kWarps && 2 << lg <= KC) ++lg;
+  const int items = n_ent << lg;
+  auto k_begin = [&](int part) { return (part * KC) >> lg; };
+  auto part_of = [&](int item) { return item & ((1 << lg) - 1); };
+  // the next stage to load (lane 0): item pi of tile pt, step pk of [.., pe)
+  int pt = static_cast<int>(blockIdx.x), pi = warp, ps = 0;
+  int pk = k_begin(part_of(warp)), pe = k_begin(part_of(warp) + 1);
+  if (items <= warp) pt = tiles;
   const uint64_t policy = evict_first_policy();
   auto issue = [&]() {
     uint8_t* dst = ring + ps * kStage;
     uint64_t* bar = &full[ps];
     mbar_arrive_expect_tx(bar, kStage);
-    if constexpr (WIDE) {  // 128 bytes x 16 rows x 2 columns
-      tma_load_4d(&tmW, bar, dst, 0, pt * 16, pk * 2, ent_e[pa], policy);
+    if constexpr (WIDE) {  // 128 bytes x 16 rows x COLS columns
+      tma_load_4d(&tmW, bar, dst, 0, pt * 16, pk * COLS, ent_e[pi >> lg], policy);
     } else {
-      tma_load_3d(&tmW, bar, dst, pk * 256, pt * 16, ent_e[pa], policy);
-      tma_load_3d(&tmW, bar, dst + 2048, pk * 256 + 128, pt * 16, ent_e[pa], policy);
+#pragma unroll
+      for (int hh = 0; hh < COLS; ++hh)
+        tma_load_3d(&tmW, bar, dst + hh * 2048, pk * kStageK + hh * 128, pt * 16, ent_e[pi >> lg], policy);
     }
-    if (++pk == KC) {
-      pk = 0;
-      if ((pa += kWarps) >= n_ent) {
-        pa = warp;
+    if (++pk == pe) {
+      if ((pi += kWarps) >= items) {
+        pi = warp;
         pt += static_cast<int>(gridDim.x);
       }
+      pk = k_begin(part_of(pi));
+      pe = k_begin(part_of(pi) + 1);
     }
     if (++ps == p.stages) ps = 0;
   };
+  int steps = 0;
+#pragma unroll 1
+  for (int i = warp; i < items; i += kWarps) steps += k_begin(part_of(i) + 1) - k_begin(part_of(i));
+  steps *= my_tiles;
   int issued = min(steps, p.stages), consumed = 0;
   if (lane == 0)
     for (int i = 0; i < issued; ++i) issue();
@@ -589,22 +609,36 @@ __global__ void __launch_bounds__(kThreads) few_down(const __grid_constant__ CUt
   uint32_t ph = 0;
   bool ok = true;
   for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    for (int a = warp; a < n_ent && ok; a += kWarps) {
+    // Thread (t, col) has the tile's column col of token t; what its first eight slots need is
+    // loaded while the products run (zeros for a slot without an expert).
+    const int t = threadIdx.x >> 4, col = threadIdx.x & 15, first = t * p.k;
+    auto scales_of = [&](int j, float& b, float& s_dn, float& w) {
+      const int e = t < p.T && j < p.k ? slot_e[first + j] : -1;
+      const bool live = e >= 0 && e < p.E;
+      b = live ? h_s[first + j] : 0.0f;
+      s_dn = live ? __ldg(p.s_dn + static_cast<int64_t>(e) * p.H + tile * 16 + col) : 0.0f;
+      w = live ? slot_w[first + j] : 0.0f;
+    };
+    float b[8], s_dn[8], w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) scales_of(j, b[j], s_dn[j], w[j]);
+#pragma unroll 1
+    for (int item = warp; item < items && ok; item += kWarps) {
+      const int a = item >> lg, k_end = k_begin(part_of(item) + 1);
       const int cnt = ent_n[a];
-      const float* sd = p.s_dn + static_cast<int64_t>(ent_e[a]) * p.H + tile * 16 + g;
-      const float s0 = __ldg(sd), s1 = __ldg(sd + 8);
       int acc[2][4] = {};
       auto run = [&](auto nt) {
         constexpr int NT = decltype(nt)::value;
         const uint8_t* x[NT];
-        int part[NT][4] = {};
+        int sum[NT][4] = {};
 #pragma unroll
         for (int i = 0; i < NT; ++i) x[i] = codes + list[a * kEntry + min(i * 8 + g, cnt - 1)] * pl.row;
-        for (int kc = 0; kc < KC; ++kc) {
+#pragma unroll 1
+        for (int kc = k_begin(part_of(item)); kc < k_end; ++kc) {
           ok = mbar_wait(&full[s], ph, &g_status, kCodeDown);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          stage_product<NT>(part, ring + s * kStage, g, q, x, kc * 256, p.I);
+          stage_product<NT, COLS>(sum, ring + s * kStage, g, q, x, kc * kStageK, p.I);
           ++consumed;
           __syncwarp();
           if (lane == 0 && issued < steps) issue();
@@ -617,36 +651,46 @@ __global__ void __launch_bounds__(kThreads) few_down(const __grid_constant__ CUt
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[i][r] = part[i][r];
+          for (int r = 0; r < 4; ++r) acc[i][r] = sum[i][r];
       };
       if (cnt <= 8) run(std::integral_constant<int, 1>{});
       else run(std::integral_constant<int, 2>{});
-      if (!ok) break;
+      // the parts' sums meet as integers: their order does not matter
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const int at = i * 8 + 2 * q + r;
           if (at < cnt) {
-            const int slot = list[a * kEntry + at];
-            const float hs = h_s[slot];
-            y[slot * 16 + g] = round_trip<T>(__fmul_rn(__fmul_rn(__int2float_rn(acc[i][r]), hs), s0));
-            y[slot * 16 + g + 8] = round_trip<T>(__fmul_rn(__fmul_rn(__int2float_rn(acc[i][2 + r]), hs), s1));
+            int* ys = y + list[a * kEntry + at] * 16 + g;
+            atomicAdd(ys, acc[i][r]);
+            atomicAdd(ys + 8, acc[i][2 + r]);
           }
         }
       }
     }
     __syncthreads();
-    {
-      const int t = threadIdx.x >> 4, col = threadIdx.x & 15;
-      if (t < p.T) {
-        float sum = 0.0f;
-        for (int j = 0; j < p.k; ++j) {
-          const int slot = t * p.k + j, e = slot_e[slot];
-          if (e >= 0 && e < p.E) sum = __fadd_rn(sum, __fmul_rn(slot_w[slot], y[slot * 16 + col]));
-        }
-        static_cast<T*>(p.out)[static_cast<int64_t>(t) * p.H + tile * 16 + col] = from_f32<T>(sum);
+    if (t < p.T) {
+      // y = T(float(sum) b s_dn) of each slot, the token's weighted sum, zeros for the next tile
+      int* ys = y + first * 16 + col;
+      int part[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) part[j] = j < p.k ? ys[j * 16] : 0;
+      float sum = 0.0f;
+      auto add = [&](int v, float b_j, float s_j, float w_j) {
+        sum = __fadd_rn(sum, __fmul_rn(w_j, round_trip<T>(__fmul_rn(__fmul_rn(__int2float_rn(v), b_j), s_j))));
+      };
+#pragma unroll
+      for (int j = 0; j < 8; ++j) add(part[j], b[j], s_dn[j], w[j]);
+#pragma unroll 1
+      for (int j = 8; j < p.k; ++j) {
+        float b_j, s_j, w_j;
+        scales_of(j, b_j, s_j, w_j);
+        add(ys[j * 16], b_j, s_j, w_j);
       }
+#pragma unroll 1
+      for (int j = 0; j < p.k; ++j) ys[j * 16] = 0;
+      static_cast<T*>(p.out)[static_cast<int64_t>(t) * p.H + tile * 16 + col] = from_f32<T>(sum);
     }
     __syncthreads();  // y is read before the next tile writes it
   }
@@ -678,20 +722,19 @@ int few_status_read_and_clear(int* code) {
 
 namespace {
 
-#ifndef FEW_MIN
-#define FEW_MIN 16384
-#endif
 constexpr int kSmemMax = 226 * 1024;  // static shared memory (the entry list's) beside it
 
-// Ring depth of a kernel: three stages a warp, two where the codes leave no room; 0: none fits.
-int few_stages(int rows, int64_t k_len, int slots, int E, int extra) {
+// Ring of a kernel: three stages a warp, two where the codes leave no room; 0: none fits.
+int few_stages(int cols, int rows, int64_t k_len, int slots, int E, int extra) {
   for (int st = 3; st >= 2; --st)
-    if (few::make_plan(st, rows, (int)k_len, slots, E, extra).total + 2048 <= kSmemMax) return st;
+    if (few::make_plan(cols, st, rows, (int)k_len, slots, E, extra).total + 2048 <= kSmemMax) return st;
   return 0;
 }
 
-// CTAs per cluster that share the preparation: with few rows it costs more than it saves.
-int few_cluster(int64_t rows, int64_t k_len) { return rows * k_len >= FEW_MIN ? 8 : 1; }
+// CTAs per cluster that share the preparation. Eight, where the rows have 16384 values in all:
+// sixteen tokens through 8 of 128 experts 64 us, 71 without clusters; fewer values are sooner
+// quantised than shared (one token of 2048: 20.9 us, in clusters 21.1).
+int few_cluster(int64_t rows, int64_t k_len) { return rows * k_len >= 16384 ? 8 : 1; }
 
 // Grid of `want` CTAs at most, in clusters of cs that are resident at once.
 int few_grid(int64_t want, int smem, int cs) {
@@ -751,44 +794,78 @@ int configure(Kern kern, std::atomic<bool>* done) {
   return FNI8_OK;
 }
 
-template <typename T, int ACT, bool WIDE_GU>
+template <typename T, int ACT, bool WIDE, int COLS>
 int launch_gate_up(const few::Layer& p, const CUtensorMap& map, int smem, cudaStream_t st) {
   static std::atomic<bool> done[kMaxDevices] = {};
-  if (int s = configure(few::few_gate_up<T, ACT, WIDE_GU>, done)) return s;
+  if (int s = configure(few::few_gate_up<T, ACT, WIDE, COLS>, done)) return s;
   const int cs = few_cluster(p.T, p.H);
   // units at most: every slot its own expert
   const int grid = few_grid((int64_t)p.T * p.k * (p.I / 8), smem, cs);
-  launch_cluster(few::few_gate_up<T, ACT, WIDE_GU>, grid, cs, smem, st, map, p);
+  launch_cluster(few::few_gate_up<T, ACT, WIDE, COLS>, grid, cs, smem, st, map, p);
   return FNI8_OK;
 }
 
-template <typename T, bool WIDE_DN>
+template <typename T, bool WIDE, int COLS>
 int launch_down(const few::Layer& p, const CUtensorMap& map, int smem, cudaStream_t st) {
   static std::atomic<bool> done[kMaxDevices] = {};
-  if (int s = configure(few::few_down<T, WIDE_DN>, done)) return s;
+  if (int s = configure(few::few_down<T, WIDE, COLS>, done)) return s;
   const int cs = few_cluster(p.T * p.k, p.I);
-  launch_cluster(few::few_down<T, WIDE_DN>, few_grid(p.H / 16, smem, cs), cs, smem, st, map, p);
+  launch_cluster(few::few_down<T, WIDE, COLS>, few_grid(p.H / 16, smem, cs), cs, smem, st, map, p);
   return FNI8_OK;
+}
+
+// Columns per stage, ring and shared memory of both kernels.
+struct FewPlan {
+  int cols_g, cols_d, stages_g, stages_d, smem_g, smem_d, early;
+};
+bool few_plan(int64_t T, int64_t H, int64_t k, int64_t E, int64_t I, FewPlan* p) {
+  const int n = (int)(T * k);
+  auto gate_up = [&](int cols) {
+    p->cols_g = cols;
+    p->stages_g = few_stages(cols, (int)T, H, n, (int)E, 0);
+    p->smem_g = few::make_plan(cols, p->stages_g, (int)T, (int)H, n, (int)E, 0).total;
+    return p->stages_g > 0;
+  };
+  auto down = [&](int cols) {
+    p->cols_d = cols;
+    p->stages_d = few_stages(cols, n, I, n, (int)E, n * 64);
+    p->smem_d = few::make_plan(cols, p->stages_d, n, (int)I, n, (int)E, n * 64).total;
+    return p->stages_d > 0;
+  };
+  // Both kernels on an SM where they fit and the weights are few: one token through 8 of 128
+  // experts (38 MB) 21 us, 23 with wide stages; through 2 of 4096 x 4096 (101 MB) 41 and 38.6.
+  p->early = 0;
+  if ((int64_t)n * 3 * H * I <= (128 << 20) && gate_up(2) && down(2) && p->smem_g + p->smem_d + 2 * 2048 <= kSmemMax) {
+    p->early = 1;
+    return true;
+  }
+  return (gate_up(4) || gate_up(2)) && (down(4) || down(2));
+}
+
+template <typename T, int ACT>
+int gate_up_any(const few::Layer& p, const FewPlan& f, const CUtensorMap& map, cudaStream_t st) {
+  if (p.H % 128 == 0)
+    return f.cols_g == 4 ? launch_gate_up<T, ACT, true, 4>(p, map, f.smem_g, st)
+                         : launch_gate_up<T, ACT, true, 2>(p, map, f.smem_g, st);
+  return f.cols_g == 4 ? launch_gate_up<T, ACT, false, 4>(p, map, f.smem_g, st)
+                       : launch_gate_up<T, ACT, false, 2>(p, map, f.smem_g, st);
 }
 
 template <typename T>
-int launch_few(const few::Layer& layer, int act, const CUtensorMap& gu, const CUtensorMap& dn, cudaStream_t st) {
+int launch_few(const few::Layer& layer, const FewPlan& f, int act, const CUtensorMap& gu, const CUtensorMap& dn,
+               cudaStream_t st) {
   few::Layer p = layer, d = layer;
-  const int slots = p.T * p.k;
-  p.stages = few_stages(p.T, p.H, slots, p.E, 0);
-  d.stages = few_stages(slots, p.I, slots, p.E, slots * 64);
-  const int sg = few::make_plan(p.stages, p.T, p.H, slots, p.E, 0).total;
-  const int sd = few::make_plan(d.stages, slots, p.I, slots, p.E, slots * 64).total;
-  p.early = d.early = sg + sd + 2 * 2048 <= kSmemMax ? 1 : 0;
-  const bool wide_gu = p.H % 128 == 0, wide_dn = p.I % 128 == 0;
-  int s;
-  if (act == FNI8_ACT_SILU)
-    s = wide_gu ? launch_gate_up<T, FNI8_ACT_SILU, true>(p, gu, sg, st) : launch_gate_up<T, FNI8_ACT_SILU, false>(p, gu, sg, st);
-  else
-    s = wide_gu ? launch_gate_up<T, FNI8_ACT_GELU_TANH, true>(p, gu, sg, st)
-                : launch_gate_up<T, FNI8_ACT_GELU_TANH, false>(p, gu, sg, st);
+  p.stages = f.stages_g;
+  d.stages = f.stages_d;
+  p.early = d.early = f.early;
+  int s = act == FNI8_ACT_SILU ? gate_up_any<T, FNI8_ACT_SILU>(p, f, gu, st)
+                               : gate_up_any<T, FNI8_ACT_GELU_TANH>(p, f, gu, st);
   if (s) return s;
-  if ((s = wide_dn ? launch_down<T, true>(d, dn, sd, st) : launch_down<T, false>(d, dn, sd, st))) return s;
+  if (d.I % 128 == 0)
+    s = f.cols_d == 4 ? launch_down<T, true, 4>(d, dn, f.smem_d, st) : launch_down<T, true, 2>(d, dn, f.smem_d, st);
+  else
+    s = f.cols_d == 4 ? launch_down<T, false, 4>(d, dn, f.smem_d, st) : launch_down<T, false, 2>(d, dn, f.smem_d, st);
+  if (s) return s;
   FNI8_CHECK_LAUNCH("moe few-token layer");
   return FNI8_OK;
 }
@@ -798,25 +875,27 @@ int launch_few(const few::Layer& layer, int act, const CUtensorMap& gu, const CU
 bool few_supported(int64_t T, int64_t H, int64_t k, int64_t E, int64_t I) {
   if (T < 1 || T > few::kMaxTokens || k < 1 || k > 32 || T * k > few::kMaxSlots || E < 1 || E > few::kMaxExperts) return false;
   if (H % 16 != 0 || I % 16 != 0 || H > (1 << 17) || I > (1 << 17)) return false;
-  const int n = (int)(T * k);
-  return few_stages((int)T, H, n, (int)E, 0) > 0 && few_stages(n, I, n, (int)E, n * 64) > 0;
+  FewPlan p;
+  return few_plan(T, H, k, E, I, &p);
 }
 
 int few_moe(const FewMoe& m, cudaStream_t st) {
+  FewPlan f;
+  if (!few_plan(m.T, m.H, m.k, m.E, m.I, &f)) return fail(FNI8_ERR_UNSUPPORTED, "few-token layer: sizes");
   // One load per stage where K is whole 128-byte columns (they become a dimension of the map);
   // small loads are issued at one in some 35 cycles, four to a stage took the first ring 1.7 us.
   CUtensorMap gu, dn;
   const uint64_t H = (uint64_t)m.H, I = (uint64_t)m.I, E = (uint64_t)m.E;
   if (m.H % 128 == 0) {
     const uint64_t dims[5] = {128, I, 2, H / 128, E}, strides[4] = {H, I * H, 128, 2 * I * H};
-    const uint32_t box[5] = {128, 8, 2, 2, 1};
+    const uint32_t box[5] = {128, 8, 2, (uint32_t)f.cols_g, 1};
     if (int s = encode_tmap_i8(&gu, m.w_gu, 5, dims, strides, box)) return s;
   } else if (int s = encode_tmap_3d_i8(&gu, m.w_gu, H, 2 * I, E, H, 2 * I * H, 128, 8)) {
     return s;
   }
   if (m.I % 128 == 0) {
     const uint64_t dims[4] = {128, H, I / 128, E}, strides[3] = {I, 128, H * I};
-    const uint32_t box[4] = {128, 16, 2, 1};
+    const uint32_t box[4] = {128, 16, (uint32_t)f.cols_d, 1};
     if (int s = encode_tmap_i8(&dn, m.w_dn, 4, dims, strides, box)) return s;
   } else if (int s = encode_tmap_3d_i8(&dn, m.w_dn, I, H, E, I, H * I, 128, 16)) {
     return s;
@@ -824,7 +903,8 @@ int few_moe(const FewMoe& m, cudaStream_t st) {
   few::Layer p{m.x, m.logits, m.topi, m.topw, m.sel_bias, (int)m.T, (int)m.H, (int)m.E, (int)m.I, (int)m.k, m.scoring,
                (int)m.n_groups, (int)m.topk_group, m.norm_topk, m.dtype, m.scaling, m.s_gu, m.s_dn, m.h, m.out, 0, 0, m.t_count, m.t_slot_e, m.t_slot_w, m.t_ent_e,
                m.t_ent_n, m.t_list};
-  return m.dtype == FNI8_F16 ? launch_few<__half>(p, m.act, gu, dn, st) : launch_few<__nv_bfloat16>(p, m.act, gu, dn, st);
+  return m.dtype == FNI8_F16 ? launch_few<__half>(p, f, m.act, gu, dn, st)
+                              : launch_few<__nv_bfloat16>(p, f, m.act, gu, dn, st);
 }
 
 }  // namespace fni8h
