@@ -533,10 +533,15 @@ int launch_tile(const Fp4Gemm& g, cudaStream_t st) {
   return FNI8_OK;
 }
 
+// 128 x 128 tiles of one CTA each where they take no more waves than 256 x 256 tiles of a pair,
+// whose waves last longer: 192 x 4096 x 4096 mxfp4 11.6 us (pairs 13.1), 333 x 12288 x 4096 18.8
+// (22.6), 512 x 1024 x 4096 nvfp4 11.3 (14.3), two waves against one 1024 x 4096 x 4096 19.0 (14.9).
 template <int FMT>
 int pick_tile(const Fp4Gemm& g, cudaStream_t st) {
-  if (g.M > 128) return launch_tile<FMT, 256, true>(g, st);
-  return launch_tile<FMT, 128, false>(g, st);
+  const int64_t sms = num_sms(current_device()), pairs = sms > 1 ? sms / 2 : 1;
+  const int64_t small = ((g.M + 127) / 128) * ((g.N + 127) / 128), large = ((g.M + 255) / 256) * ((g.N + 255) / 256);
+  if ((small + sms - 1) / sms <= (large + pairs - 1) / pairs) return launch_tile<FMT, 128, false>(g, st);
+  return launch_tile<FMT, 256, true>(g, st);
 }
 
 int run_gemm(const Fp4Gemm& g, cudaStream_t st) {
