@@ -1,11 +1,11 @@
-// Decode GEMM of 4-bit floating point operands (1 to 128 tokens): every SM streams weights.
+// GEMM of 4-bit floating point operands for few tokens or few tiles: every SM streams weights.
 //
 //   acc^T[n, m] = sum_k w[n,k] sw[n,k/g] a[m,k] sa[m,k/g]   (tcgen05.mma kind::mxf4 / mxf4nvf4)
 //   out[m, n]   = dtype(acc * ra[m] * rw[n] (+ bias[n]))
 //
 // Bound: HBM, N K (1/2 + 1/g) bytes of weights read once. As in gemm_splitk.cu the operands
 // are swapped (128 weight rows = MMA M, NT tokens = MMA N) and a cluster of S CTAs splits the
-// K range of a weight tile, S chosen so that the grid fills the GPU once; weights are loaded
+// K range of a weight tile (and of a block of 128 tokens, where there are more), S chosen so that the grid fills the GPU once; weights are loaded
 // before the wait for the quantiser. Here the S partial accumulators meet in shared memory:
 // CTA r owns a share of the token columns, every CTA stores the columns of the others into
 // their landing areas (distributed shared memory, 16-byte pieces of four tokens, the weight row
@@ -164,7 +164,7 @@ __device__ __forceinline__ void quantise_slice(const Epi& epi, int M, int kbeg, 
 template <int FMT, int NT, bool FUSED>
 __global__ void __launch_bounds__(kThreads, 2)
     fp4_splitk_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
-                      const __grid_constant__ CUtensorMap tmSW, const __grid_constant__ CUtensorMap tmSX, Epi epi, int M,
+                      const __grid_constant__ CUtensorMap tmSW, const __grid_constant__ CUtensorMap tmSX, Epi epi, int rows,
                       int N, int Kp, int ktiles, int stages, int xstages) {
   using C = Cfg<FMT, NT, FUSED>;
   extern __shared__ uint8_t smem_raw[];
@@ -185,6 +185,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank()), S = static_cast<int>(cluster_nctarank());
   const int tile = static_cast<int>(blockIdx.x) / S;
+  const int m0 = static_cast<int>(blockIdx.y) * NT, M = min(rows - m0, NT);  // this CTA's tokens
   const int kb = (Kp + 255) / 256;
   const int kbeg = static_cast<int>(static_cast<int64_t>(rank) * kb / S);
   const int nk = static_cast<int>(static_cast<int64_t>(rank + 1) * kb / S) - kbeg;
@@ -233,8 +234,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       auto load_x = [&](int s, int k) {
         if constexpr (!FUSED) {
           uint8_t* dst = smem + s * C::STAGE + C::W_BYTES + C::SF_BYTES;
-          tma_load_2d(&tmSX, &full[s], dst, 0, k * C::TILES * 4);
-          tma_load_2d(&tmX, &full[s], dst + C::SF_BYTES, k * 128, 0);
+          tma_load_2d(&tmSX, &full[s], dst, 0, (static_cast<int>(blockIdx.y) * ktiles + k * C::TILES) * 4);
+          tma_load_2d(&tmX, &full[s], dst + C::SF_BYTES, k * 128, m0);
         }
       };
       const int pre = nk < stages ? nk : stages;
@@ -304,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       __syncwarp();
       if (lane == 0) mbar_arrive(xready);
     } else if constexpr (FMT == FNI8_NVFP4) {
-      for (int m = threadIdx.x - 64; m < M; m += 128) s_ra[m] = __ldg(epi.a_rs + m);
+      for (int m = threadIdx.x - 64; m < M; m += 128) s_ra[m] = __ldg(epi.a_rs + m0 + m);
       named_bar_sync(1, 128);
     }
     if (lane == 0) okt = mbar_wait(tfull, 0, &g_status, kCodeEpilogue) ? 1 : 0;
@@ -379,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           float o = v[j];
           if constexpr (FMT == FNI8_NVFP4) o = __fmul_rn(__fmul_rn(o, s_ra[m]), rw);
           if (epi.bias != nullptr) o = __fadd_rn(o, bias);
-          const int64_t at = static_cast<int64_t>(m) * N + n;
+          const int64_t at = static_cast<int64_t>(m0 + m) * N + n;
           if (epi.bf16) static_cast<__nv_bfloat16*>(epi.out)[at] = __float2bfloat16_rn(o);
           else static_cast<__half*>(epi.out)[at] = __float2half_rn(o);
         }
@@ -436,11 +437,11 @@ struct Plan {
 };
 
 // Ring: half an SM's shared memory where that holds kMinRing stages beside the rest (two CTAs
-// per SM), else a whole SM's. S: as many CTAs per weight tile as are resident at once.
+// per SM), else a whole SM's. S: as many CTAs per tile as are resident at once.
 template <int FMT, int NT, bool FUSED>
-Plan plan_splitk(int64_t M, int64_t N, int64_t K) {
+Plan plan_splitk(int64_t rows, int64_t N, int64_t K) {
   using C = fp4s::Cfg<FMT, NT, FUSED>;
-  const int64_t tiles = (N + 127) / 128;
+  const int64_t tiles = (N + 127) / 128 * ((rows + NT - 1) / NT), M = rows < NT ? rows : NT;
   const int kb = (int)((fp4::padded_k(K) + 255) / 256);
   auto plan = [&](int S) {
     const int land = S > 1 ? S * fp4s::column_share(((int)M + 3) & ~3, S) * 128 * 4 : 0;
@@ -495,7 +496,7 @@ int launch_splitk(const Fp4Gemm& g, const void* x, cudaStream_t st) {
   }
   const fp4s::Epi epi{x, g.K, g.a_rs, g.w_rs, g.bias, g.out, g.bf16 ? 1 : 0};
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((g.N + 127) / 128 * p.S));
+  cfg.gridDim = dim3((unsigned)((g.N + 127) / 128 * p.S), (unsigned)((g.M + NT - 1) / NT));
   cfg.blockDim = dim3(fp4s::kThreads);
   cfg.dynamicSmemBytes = p.smem;
   cfg.stream = st;
@@ -526,6 +527,12 @@ int splitk_any(const Fp4Gemm& g, cudaStream_t st) {
 
 int fp4_splitk(const Fp4Gemm& g, cudaStream_t st) {
   return g.format == FNI8_MXFP4 ? splitk_any<FNI8_MXFP4>(g, st) : splitk_any<FNI8_NVFP4>(g, st);
+}
+
+int fp4_splitk_parts(const Fp4Gemm& g) {
+  const Plan p = g.format == FNI8_MXFP4 ? plan_splitk<FNI8_MXFP4, 128, false>(g.M, g.N, g.K)
+                                        : plan_splitk<FNI8_NVFP4, 128, false>(g.M, g.N, g.K);
+  return p.fits ? p.S : 1;
 }
 
 bool fp4_fused_supported(int format, int64_t M, int64_t N, int64_t K) {

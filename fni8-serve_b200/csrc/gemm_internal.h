@@ -99,8 +99,9 @@ int fp4_check_rows(const void* x, int dtype, int format, int64_t M, int64_t K, c
 // pad: also zero the scales of the rows behind M in the last tile.
 int fp4_quantize(const void* x, int dtype, int format, int64_t M, int64_t K, bool pad, uint8_t* q, uint8_t* sf,
                  float* row_scale, cudaStream_t st);
-// The swap-AB split-K kernel for M <= 128 (gemm_fp4_splitk.cu).
+// The swap-AB split-K kernel (gemm_fp4_splitk.cu), and into how many parts it would cut K at M > 64.
 int fp4_splitk(const Fp4Gemm& g, cudaStream_t st);
+int fp4_splitk_parts(const Fp4Gemm& g);
 // Its form that quantises the 16-bit rows x itself (16-byte aligned; a, a_sf and a_rs unused).
 bool fp4_fused_supported(int format, int64_t M, int64_t N, int64_t K);
 int fp4_fused(const Fp4Gemm& g, const void* x, cudaStream_t st);

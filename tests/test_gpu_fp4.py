@@ -158,7 +158,8 @@ def random_qt(N, K, scheme, seed, exact):
 
 SHAPES = [(1, 8, 32), (1, 1, 1), (2, 129, 64), (3, 200, 96), (16, 256, 256), (17, 130, 320), (33, 1030, 288), (64, 128, 4096),
           (100, 384, 1000), (128, 512, 2048), (129, 640, 512), (200, 77, 130), (256, 1024, 1024), (300, 264, 2080),
-          (513, 520, 736), (1100, 2056, 544)]
+          (513, 520, 736), (1100, 2056, 544), (100, 300, 4100), (65, 128, 9000), (129, 130, 4096), (300, 1030, 6000),
+          (513, 129, 4097), (120, 19000, 300), (300, 13000, 70), (1000, 4200, 328), (128, 40000, 96)]
 
 
 @pytest.mark.parametrize("scheme", SCHEMES)
