@@ -382,9 +382,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     __syncwarp();
   } else {
     // ------------------------------------------------------------ epilogue
-    // Warp w reads the TMEM lanes [32 q, 32 q + 32), q = w % 4, and half of the columns. All
-    // of its outputs are formed in registers first, which frees the accumulator for the next
-    // tile before they are stored.
+    // Warp w reads the TMEM lanes [32 q, 32 q + 32), q = w % 4, and half of the columns, all of
+    // them before anything else is done: the next tile's MMAs wait for the accumulator.
     const int q = warp & 3, ew = warp - 2, et = threadIdx.x - 64;
     const int c_beg = (ew >> 2) * (BN / 2);
     float* s_rw = reinterpret_cast<float*>(stg + kEpiWarps * C::STG_BUF);
@@ -420,19 +419,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       named_bar_sync(2, kEpiThreads);
       const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BN + c_beg);
       constexpr int kChunks = BN / 64;
-      uint4 o[kChunks][4];
-      uint32_t r[32];
-      tmem_ld32(tb, r);
+      uint32_t r[kChunks][32];
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        tmem_ld_wait();
-        tmem_regs_ready(r);
-        const float* w = s_rw + c_beg + c * 32;
-        const float* b = s_bias + c_beg + c * 32;
-        if (epi.bf16) finish_chunk<__nv_bfloat16, FMT>(r, ra, w, b, epi.bias != nullptr, o[c]);
-        else finish_chunk<__half, FMT>(r, ra, w, b, epi.bias != nullptr, o[c]);
-        if (c + 1 < kChunks) tmem_ld32(tb + (c + 1) * 32, r);
-      }
+      for (int c = 0; c < kChunks; ++c) tmem_ld32(tb + c * 32, r[c]);
+      tmem_ld_wait();
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) tmem_regs_ready(r[c]);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
@@ -442,9 +434,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
         const int n0 = nb * BN + c_beg + c * 32;
-        if (rows > 0 && n0 < N)
-          store_slab(stg + ew * C::STG_BUF, o[c], lane, &tmOut, epi.tma_store != 0, static_cast<uint16_t*>(epi.out), n0,
+        if (rows > 0 && n0 < N) {
+          const float* w = s_rw + c_beg + c * 32;
+          const float* b = s_bias + c_beg + c * 32;
+          uint4 o[4];
+          if (epi.bf16) finish_chunk<__nv_bfloat16, FMT>(r[c], ra, w, b, epi.bias != nullptr, o);
+          else finish_chunk<__half, FMT>(r[c], ra, w, b, epi.bias != nullptr, o);
+          store_slab(stg + ew * C::STG_BUF, o, lane, &tmOut, epi.tma_store != 0, static_cast<uint16_t*>(epi.out), n0,
                      N, row0, rows);
+        }
       }
       if (++acc == C::NACC) {
         acc = 0;
