@@ -68,17 +68,19 @@ __device__ __forceinline__ uint32_t raw_max(const Raw16& r) {
 }
 
 // GROUP threads per row. KEEP: chunks of a row that each thread holds in registers (0: the
-// row is read a second time, for longer ones). Rows [M, pad_rows) only get zero scales.
+// row is read a second time, for longer ones). Rows [M, pad_rows) only get zero scales. early:
+// the next kernel may start at once. It must not where the rows may be weights: the GEMMs load
+// those before they wait for the kernel in front of them.
 template <typename T, int FMT, int VW, int GROUP, int KEEP>
 __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP) quant_rows(const T* __restrict__ x, int64_t M, int64_t K,
                                                                         int64_t pad_rows, uint8_t* __restrict__ q,
                                                                         uint8_t* __restrict__ sf,
-                                                                        float* __restrict__ row_scale) {
+                                                                        float* __restrict__ row_scale, bool early) {
   constexpr int kThreads = GROUP < 128 ? 128 : GROUP;
   constexpr int kLanes = Fmt<FMT>::kBlock / 16;  // threads that share a block
   constexpr int kWordLanes = 4 * kLanes;         // threads that share a cell of four scales
   __shared__ uint32_t red[kThreads / 32];
-  pdl_launch_dependents();
+  if (early) pdl_launch_dependents();
   pdl_wait();
   const int g = threadIdx.x / GROUP, t = threadIdx.x % GROUP, lane = threadIdx.x & 31;
   const int64_t tiles = k_tiles(FMT, K);
@@ -232,13 +234,13 @@ int check_fp4_rows(int format, int64_t M, int64_t K, const char* what) {
 }
 
 template <typename T, int FMT, int VW>
-void launch_quant(const T* x, int64_t M, int64_t K, int64_t pad_rows, uint8_t* q, uint8_t* sf, float* rs,
+void launch_quant(const T* x, int64_t M, int64_t K, int64_t pad_rows, bool early, uint8_t* q, uint8_t* sf, float* rs,
                   cudaStream_t st) {
   const int64_t chunks = fp4::k_tiles(FMT, K) * 4 * (fp4::Fmt<FMT>::kBlock / 16);
   const int64_t blocks = chunks <= 64 ? (pad_rows + 3) / 4 : pad_rows;
   const dim3 grid((unsigned)(blocks < 148 * 64 ? blocks : 148 * 64));
 #define FNI8_QUANT_FP4(G, KEEP)                                                                                     \
-  launch_pdl(fp4::quant_rows<T, FMT, VW, G, KEEP>, grid, dim3(G < 128 ? 128 : G), 0, st, x, M, K, pad_rows, q, sf, rs)
+  launch_pdl(fp4::quant_rows<T, FMT, VW, G, KEEP>, grid, dim3(G < 128 ? 128 : G), 0, st, x, M, K, pad_rows, q, sf, rs, early)
   // few long rows: more threads to each (1 x 12288 nvfp4 2.9 us with 512, 7.7 with 128)
   const bool few = M < 4 * 148;
   if constexpr (FMT == FNI8_MXFP4) {  // no row maximum: nothing to keep
@@ -259,14 +261,14 @@ void launch_quant(const T* x, int64_t M, int64_t K, int64_t pad_rows, uint8_t* q
 }
 
 template <typename T, int FMT>
-void launch_quant_vw(const void* x, int64_t M, int64_t K, int64_t pad_rows, uint8_t* q, uint8_t* sf, float* rs,
+void launch_quant_vw(const void* x, int64_t M, int64_t K, int64_t pad_rows, bool early, uint8_t* q, uint8_t* sf, float* rs,
                      cudaStream_t st) {
   const T* xt = static_cast<const T*>(x);
   const uintptr_t a = reinterpret_cast<uintptr_t>(x) | (M > 1 ? static_cast<uintptr_t>(K) * 2 : 0);
-  if (a % 16 == 0) launch_quant<T, FMT, 8>(xt, M, K, pad_rows, q, sf, rs, st);
-  else if (a % 8 == 0) launch_quant<T, FMT, 4>(xt, M, K, pad_rows, q, sf, rs, st);
-  else if (a % 4 == 0) launch_quant<T, FMT, 2>(xt, M, K, pad_rows, q, sf, rs, st);
-  else launch_quant<T, FMT, 1>(xt, M, K, pad_rows, q, sf, rs, st);
+  if (a % 16 == 0) launch_quant<T, FMT, 8>(xt, M, K, pad_rows, early, q, sf, rs, st);
+  else if (a % 8 == 0) launch_quant<T, FMT, 4>(xt, M, K, pad_rows, early, q, sf, rs, st);
+  else if (a % 4 == 0) launch_quant<T, FMT, 2>(xt, M, K, pad_rows, early, q, sf, rs, st);
+  else launch_quant<T, FMT, 1>(xt, M, K, pad_rows, early, q, sf, rs, st);
 }
 
 }  // namespace
@@ -277,11 +279,11 @@ int fp4_quantize(const void* x, int dtype, int format, int64_t M, int64_t K, boo
                  float* row_scale, cudaStream_t st) {
   const int64_t pad_rows = pad ? fp4::row_tiles(M) * 128 : M;
   if (format == FNI8_MXFP4) {
-    if (dtype == FNI8_F16) launch_quant_vw<__half, FNI8_MXFP4>(x, M, K, pad_rows, q, sf, row_scale, st);
-    else launch_quant_vw<__nv_bfloat16, FNI8_MXFP4>(x, M, K, pad_rows, q, sf, row_scale, st);
+    if (dtype == FNI8_F16) launch_quant_vw<__half, FNI8_MXFP4>(x, M, K, pad_rows, !pad, q, sf, row_scale, st);
+    else launch_quant_vw<__nv_bfloat16, FNI8_MXFP4>(x, M, K, pad_rows, !pad, q, sf, row_scale, st);
   } else {
-    if (dtype == FNI8_F16) launch_quant_vw<__half, FNI8_NVFP4>(x, M, K, pad_rows, q, sf, row_scale, st);
-    else launch_quant_vw<__nv_bfloat16, FNI8_NVFP4>(x, M, K, pad_rows, q, sf, row_scale, st);
+    if (dtype == FNI8_F16) launch_quant_vw<__half, FNI8_NVFP4>(x, M, K, pad_rows, !pad, q, sf, row_scale, st);
+    else launch_quant_vw<__nv_bfloat16, FNI8_NVFP4>(x, M, K, pad_rows, !pad, q, sf, row_scale, st);
   }
   FNI8_CHECK_LAUNCH("quantize_rows_fp4");
   return FNI8_OK;

@@ -292,13 +292,12 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_wait(drain, 0, &g_status, kCodeDrain);
     }
   } else {
-    if (n < N) {
-      if constexpr (FMT == FNI8_NVFP4) rw = __ldg(epi.w_rs + n);
-      if (epi.bias != nullptr)
-        bias = epi.bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(epi.bias)[n])
-                        : __half2float(static_cast<const __half*>(epi.bias)[n]);
-    }
+    if constexpr (FMT == FNI8_NVFP4)
+      if (n < N) rw = __ldg(epi.w_rs + n);
     pdl_wait();
+    if (n < N && epi.bias != nullptr)
+      bias = epi.bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(epi.bias)[n])
+                      : __half2float(static_cast<const __half*>(epi.bias)[n]);
     if constexpr (FUSED) {
       if (epi.bf16) quantise_slice<FMT, NT, __nv_bfloat16>(epi, M, kbeg, nk, rank, S, xs, tops + 128, tops, s_ra, posted);
       else quantise_slice<FMT, NT, __half>(epi, M, kbeg, nk, rank, S, xs, tops + 128, tops, s_ra, posted);

@@ -330,3 +330,24 @@ def test_linear_in_one_kernel(scheme, dtype, M, N, K):
     flat[1:] = x.reshape(-1)
     assert torch.equal(fni8.linear(flat[1:].view(M, K), w, bias=bias), want)
     assert fni8.device_status() == 0
+
+
+@pytest.mark.parametrize("scheme", SCHEMES)
+@pytest.mark.parametrize("M", [1, 40, 300])
+def test_weights_quantised_right_before(scheme, M):
+    """linear directly behind the kernel that writes its weights, on the memory that the last weights had."""
+    import fni8
+
+    N, K = 12288, 4096
+    x = torch.randn(M, K, generator=gen(1)).half().to(DEV)
+    ws = [0.05 * torch.randn(N, K, device=DEV, dtype=torch.float16) * (i + 1) for i in range(4)]
+    torch.cuda.synchronize()
+    got = []
+    for w in ws:
+        q = fni8.quantize_fp4(w, scheme)
+        got.append(fni8.linear(x, q))
+        del q
+    for w, y in zip(ws, got):
+        q = fni8.quantize_fp4(w, scheme)
+        torch.cuda.synchronize()
+        assert torch.equal(fni8.linear(x, q), y)
