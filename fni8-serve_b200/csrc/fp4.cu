@@ -49,22 +49,8 @@ __device__ __forceinline__ Raw16 load16(const T* __restrict__ row, int64_t k, in
 }
 
 template <typename T>
-__device__ __forceinline__ void unpack8(const uint4& u, float (&f)[8]) {
-  const T* v = reinterpret_cast<const T*>(&u);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = to_f32<T>(v[i]);
-}
-
-// Largest magnitude as the bits of a float (an infinity or NaN wins): the order of the 16-bit
-// patterns without their signs.
-template <typename T>
 __device__ __forceinline__ uint32_t raw_max(const Raw16& r) {
-  auto four = [](const uint4& u) {
-    return __vmaxu2(__vmaxu2(u.x & 0x7FFF7FFFu, u.y & 0x7FFF7FFFu), __vmaxu2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu));
-  };
-  const uint32_t m = __vmaxu2(four(r.lo), four(r.hi));
-  const unsigned short top = static_cast<unsigned short>(max(m & 0xFFFFu, m >> 16));
-  return __float_as_uint(to_f32<T>(*reinterpret_cast<const T*>(&top)));
+  return pattern_bits<T>(max(pattern_max(r.lo), pattern_max(r.hi)));
 }
 
 // GROUP threads per row. KEEP: chunks of a row that each thread holds in registers (0: the
@@ -97,25 +83,27 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP) quant_rows(const T*
     uint8_t* sr = sf + (row >> 7) * tiles * 512 + row_byte(static_cast<int>(row & 127));
     int row_exp = 0;
     Raw16 kept[KEEP > 0 ? KEEP : 1];
+    uint32_t tops[KEEP > 0 ? KEEP : 1];
     if constexpr (KEEP > 0) {
 #pragma unroll
       for (int i = 0; i < KEEP; ++i)
         kept[i] = real ? load16<T, VW>(xr, static_cast<int64_t>(t + i * GROUP) * 16, K) : zero;
+#pragma unroll
+      for (int i = 0; i < KEEP; ++i) tops[i] = raw_max<T>(kept[i]);
     }
     if constexpr (FMT == FNI8_NVFP4) {
       // the row's largest finite block: a block with an infinity or NaN stands for itself alone
       uint32_t top = 0;
-      auto enter = [&](const Raw16& r) {
-        const uint32_t m = raw_max<T>(r);
+      auto enter = [&](uint32_t m) {
         if (m < kInfBits) top = max(top, m);
       };
       if constexpr (KEEP > 0) {
 #pragma unroll
-        for (int i = 0; i < KEEP; ++i) enter(kept[i]);
+        for (int i = 0; i < KEEP; ++i) enter(tops[i]);
       } else {
 #pragma unroll 2
         for (int c0 = 0; c0 < chunks; c0 += GROUP)
-          enter(real ? load16<T, VW>(xr, static_cast<int64_t>(c0 + t) * 16, K) : zero);
+          enter(raw_max<T>(real ? load16<T, VW>(xr, static_cast<int64_t>(c0 + t) * 16, K) : zero));
       }
       top = __reduce_max_sync(0xffffffffu, top);
       if constexpr (GROUP > 32) {
@@ -128,15 +116,10 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP) quant_rows(const T*
       row_exp = row_exponent(top);
       if (real && t == 0) row_scale[row] = pow2f(row_exp);
     }
-    auto emit = [&](int c, const Raw16& r) {
-      uint32_t top = raw_max<T>(r);
+    auto emit = [&](int c, const Raw16& r, uint32_t top) {
       if constexpr (kLanes == 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       const BlockScale<FMT> scale(top, row_exp);
-      float f[8];
-      unpack8<T>(r.lo, f);
-      const uint32_t lo = scale.codes(f);
-      unpack8<T>(r.hi, f);
-      const uint32_t hi = scale.codes(f);
+      const uint32_t lo = scale.template codes<T>(r.lo), hi = scale.template codes<T>(r.hi);
       // the cell's four scale bytes, from its blocks' lanes
       uint32_t word = real ? scale.byte << (8 * ((lane / kLanes) & 3)) : 0u;
 #pragma unroll
@@ -148,11 +131,13 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP) quant_rows(const T*
     if constexpr (KEEP > 0) {
 #pragma unroll
       for (int i = 0; i < KEEP; ++i)
-        if (i * GROUP < chunks) emit(t + i * GROUP, kept[i]);
+        if (i * GROUP < chunks) emit(t + i * GROUP, kept[i], tops[i]);
     } else {
 #pragma unroll 2
-      for (int c0 = 0; c0 < chunks; c0 += GROUP)
-        emit(c0 + t, real ? load16<T, VW>(xr, static_cast<int64_t>(c0 + t) * 16, K) : zero);
+      for (int c0 = 0; c0 < chunks; c0 += GROUP) {
+        const Raw16 r = real ? load16<T, VW>(xr, static_cast<int64_t>(c0 + t) * 16, K) : zero;
+        emit(c0 + t, r, raw_max<T>(r));
+      }
     }
   }
 }
@@ -166,39 +151,51 @@ __global__ void __launch_bounds__(256) dequant_rows(const uint8_t* __restrict__ 
                                                     T* __restrict__ out) {
   pdl_launch_dependents();
   pdl_wait();
-  const int per_row = static_cast<int>((K + 7) / 8);
+  constexpr int kChunks = Fmt<FMT>::kBlock / 8;  // threads that share a block
   const int64_t tiles = k_tiles(FMT, K), row_bytes = padded_k(K) / 2;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; row < M;
        row += static_cast<int64_t>(gridDim.x) * blockDim.y) {
     const float rs = FMT == FNI8_NVFP4 ? __ldg(row_scale + row) : 1.0f;
     const uint8_t* sr = sf + (row >> 7) * tiles * 512 + row_byte(static_cast<int>(row & 127));
-    const uint32_t* qr = reinterpret_cast<const uint32_t*>(q + row * row_bytes);
-#pragma unroll 4
-    for (int c = threadIdx.x; c < per_row; c += blockDim.x) {
-      const uint32_t w = __ldg(qr + c);
-      const int s = c / (Fmt<FMT>::kBlock / 8);
-      const uint32_t sb = __ldg(sr + static_cast<int64_t>(s >> 2) * 512 + (s & 3));
-      float sc;
-      if constexpr (FMT == FNI8_MXFP4) sc = sb == 0xFF ? __uint_as_float(0x7FC00000u) : pow2f(static_cast<int>(sb) - 127);
-      else sc = e4m3_value(sb);
+    // of this thread's steps, `blockDim.x` (a power of two >= 32) chunks apart
+    const uint32_t* qp = reinterpret_cast<const uint32_t*>(q + row * row_bytes) + threadIdx.x;
+    const int s0 = threadIdx.x / kChunks;  // its block of the row
+    const uint8_t* sp = sr + (s0 >> 2) * 512 + (s0 & 3);
+    const int s_step = blockDim.x / (4 * kChunks) * 512;
+    T* o = out + row * K + threadIdx.x * 8;
+    auto step = [&](int c, auto whole) {
+      uint32_t h[4];
+      e2m1x8_values(__ldg(qp), h);
+      const uint32_t sb = __ldg(sp);
+      Pair sc;
+      if constexpr (FMT == FNI8_MXFP4) {
+        const float f = sb == 0xFF ? __uint_as_float(0x7FC00000u) : pow2f(static_cast<int>(sb) - 127);
+        sc = pair(f, f);
+      } else {  // code * scale is exact in halves: 2 + 4 significant bits, between 2^-10 and 2688
+        const __half2 s2 = __half2half2(__float2half_rn(e4m3_value(sb)));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&h[i]), s2);
+          h[i] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+        sc = pair(rs, rs);
+      }
       alignas(16) T v[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        uint32_t h2;
-        asm("{\n\t.reg .b8 t;\n\tcvt.u8.u16 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}"
-            : "=r"(h2)
-            : "h"(static_cast<uint16_t>((w >> (8 * i)) & 0xFF)));
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float f = __half2float(__ushort_as_half(static_cast<unsigned short>(h2 >> (16 * j))));
-          f = __fmul_rn(f, sc);  // exact: 2 + 4 significant bits
-          if constexpr (FMT == FNI8_NVFP4) f = __fmul_rn(f, rs);
-          if constexpr (sizeof(T) == 4) v[2 * i + j] = f;
-          else v[2 * i + j] = from_f32<T>(f);
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+        float lo, hi;
+        unpair(mul2(pair(f.x, f.y), sc), lo, hi);
+        if constexpr (sizeof(T) == 4) {
+          v[2 * i] = lo;
+          v[2 * i + 1] = hi;
+        } else if constexpr (std::is_same<T, __half>::value) {
+          *reinterpret_cast<__half2*>(v + 2 * i) = __floats2half2_rn(lo, hi);
+        } else {
+          *reinterpret_cast<__nv_bfloat162*>(v + 2 * i) = __floats2bfloat162_rn(lo, hi);
         }
       }
-      T* o = out + row * K + c * 8;
-      if (c * 8 + 8 <= K) {
+      if constexpr (decltype(whole)::value) {
         char* ob = reinterpret_cast<char*>(o);
         const char* vb = reinterpret_cast<const char*>(v);
 #pragma unroll
@@ -213,7 +210,14 @@ __global__ void __launch_bounds__(256) dequant_rows(const uint8_t* __restrict__ 
         for (int i = 0; i < 8; ++i)
           if (c * 8 + i < K) o[i] = v[i];
       }
-    }
+      qp += blockDim.x;
+      sp += s_step;
+      o += blockDim.x * 8;
+    };
+    int c = threadIdx.x;
+#pragma unroll 4
+    for (; c < K >> 3; c += blockDim.x) step(c, std::true_type{});
+    if (c * 8 < K) step(c, std::false_type{});
   }
 }
 

@@ -11,6 +11,8 @@
 // tcgen05.cp.32x128b.warpx4 brings a tile into tensor memory, four scales of a row in one
 // 32-bit cell. Scales behind K are zero, so the padded part of a tile adds nothing.
 #pragma once
+#include <type_traits>
+
 #include "fni8_common.cuh"
 
 namespace fni8b {
@@ -127,12 +129,18 @@ __device__ __forceinline__ void stage_mmas(uint32_t d, const void* sa, const voi
 }
 
 // ---------------------------------------------------------------- quantisation of a chunk
-// Largest magnitude of eight values, as the bits of a float: an infinity or NaN wins.
-__device__ __forceinline__ uint32_t abs_max8(const float (&f)[8]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7FFFFFFFu);
-  return m;
+// Largest magnitude of eight 16-bit values as a 16-bit pattern (an infinity or NaN wins): the
+// order of the patterns without their signs.
+__device__ __forceinline__ uint32_t pattern_max(const uint4& u) {
+  const uint32_t m = __vmaxu2(__vmaxu2(u.x & 0x7FFF7FFFu, u.y & 0x7FFF7FFFu),
+                              __vmaxu2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu));
+  return max(m & 0xFFFFu, m >> 16);
+}
+// ... as the bits of the float
+template <typename T>
+__device__ __forceinline__ uint32_t pattern_bits(uint32_t pattern) {
+  const unsigned short top = static_cast<unsigned short>(pattern);
+  return __float_as_uint(to_f32<T>(*reinterpret_cast<const T*>(&top)));
 }
 
 // 2^e of a float, e in [-127, 127]
@@ -146,7 +154,31 @@ __device__ __forceinline__ int floor_log2(uint32_t bits) {
   return e > 0 ? e - 127 : -118 - __clz(bits);  // denormal: 2^-149 has one bit, 31 leading zeros
 }
 
-__device__ __forceinline__ uint32_t e2m1x8(const float (&f)[8]) {
+// Two floats in one register pair: the pair's product and fused multiply-add are one instruction.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair(float a, float b) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+  return p;
+}
+__device__ __forceinline__ void unpair(Pair p, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+
+__device__ __forceinline__ uint32_t e2m1x8(const Pair (&v)[4]) {
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) unpair(v[i], f[2 * i], f[2 * i + 1]);
   uint32_t out;
   asm("{\n\t.reg .b8 a, b, c, d;\n\t"
       "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
@@ -157,6 +189,18 @@ __device__ __forceinline__ uint32_t e2m1x8(const float (&f)[8]) {
       : "=r"(out)
       : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]));
   return out;
+}
+
+// Eight codes (a register) as halves: exact.
+__device__ __forceinline__ void e2m1x8_values(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "mov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
 }
 
 __device__ __forceinline__ uint32_t e4m3_bits(float v) {
@@ -205,25 +249,33 @@ struct BlockScale {
     }
   }
 
-  // Eight values' codes. nvfp4: q = f inv is the quotient but for a few units in the last
-  // place; its fused remainder f - q d is exact and corrects it to the quotient's rounding
-  // (Markstein's step, as in div_by_ge1).
-  __device__ __forceinline__ uint32_t codes(float (&f)[8]) const {
-    if constexpr (FMT == FNI8_MXFP4) {
+  // The codes of eight 16-bit values f. nvfp4: q = f inv is the quotient but for a few units in
+  // the last place; its fused remainder f - q d is exact and corrects it to the quotient's rounding
+  // (Markstein's step, as in div_by_ge1). All from -f and -inv: so a zero keeps its sign.
+  template <typename T>
+  __device__ __forceinline__ uint32_t codes(const uint4& raw) const {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    const Pair inv2 = pair(-inv, -inv), d2 = pair(d, d);
+    Pair v[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(f[i], inv);
-    } else {
-      if (pre != 1.0f) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(f[i], pre);
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t n = w[i] ^ 0x80008000u;
+      Pair f;
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        f = pair(__uint_as_float(n << 16), __uint_as_float(n & 0xFFFF0000u));
+      } else {
+        const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&n));
+        f = pair(h.x, h.y);
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float q = __fmul_rn(f[i], inv);
-        f[i] = __fmaf_rn(-__fmaf_rn(q, d, -f[i]), inv, q);  // (in this order a zero keeps its sign)
+      if constexpr (FMT == FNI8_NVFP4) {
+        if (pre != 1.0f) f = mul2(f, pair(pre, pre));
+        const Pair q = mul2(f, inv2);
+        v[i] = fma2(fma2(q, d2, f), inv2, q);
+      } else {
+        v[i] = mul2(f, inv2);
       }
     }
-    return e2m1x8(f);
+    return e2m1x8(v);
   }
 };
 

@@ -88,16 +88,11 @@ __device__ __forceinline__ void quantise_slice(const Epi& epi, int M, int kbeg, 
     raw[b] = make_uint4(0, 0, 0, 0);
     if (c * 8 < left) raw[b] = __ldg(reinterpret_cast<const uint4*>(x + m * epi.K + c * 8));  // K % 8 == 0
   }
-  auto unpack = [&](int b, float (&f)[8]) {
-    const T* v = reinterpret_cast<const T*>(&raw[b]);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = to_f32<T>(v[j]);
-  };
-  auto block_top = [&](const float (&f)[8]) {
-    uint32_t m = abs_max8(f);
+  auto block_top = [&](int b) {
+    uint32_t m = pattern_max(raw[b]);
 #pragma unroll
     for (int o = 1; o < kLanes; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    return m;
+    return pattern_bits<T>(m);
   };
   if constexpr (FMT == FNI8_NVFP4) {
     if (et < 16) s_top[et] = 0;
@@ -105,9 +100,7 @@ __device__ __forceinline__ void quantise_slice(const Epi& epi, int M, int kbeg, 
 #pragma unroll
     for (int b = 0; b < kFusedChunks; ++b) {
       if (et + 128 * b >= items) break;
-      float f[8];
-      unpack(b, f);
-      uint32_t top = block_top(f);
+      uint32_t top = block_top(b);
       if (top >= kInfBits) top = 0;  // a block with an infinity or NaN stands for itself alone
 #pragma unroll
       for (int o = kLanes; o < 32; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -147,12 +140,10 @@ __device__ __forceinline__ void quantise_slice(const Epi& epi, int M, int kbeg, 
     const int i = et + 128 * b;
     if (i >= items) break;
     const int m = i / per_row, c = i - m * per_row;
-    float f[8];
-    unpack(b, f);
-    const uint32_t top = block_top(f);
+    const uint32_t top = block_top(b);
     const int row_exp = FMT == FNI8_NVFP4 ? static_cast<int>(__float_as_uint(s_ra[m]) >> 23) - 127 : 0;
     const BlockScale<FMT> scale(top, row_exp);
-    const uint32_t codes = scale.codes(f);
+    const uint32_t codes = scale.template codes<T>(raw[b]);
     uint8_t* st = xs + (c >> 5) * C::X_STAGE;
     *reinterpret_cast<uint32_t*>(st + m * 128 + ((((c & 31) >> 2) ^ (m & 7)) << 4) + (c & 3) * 4) = codes;
     const int s = (c & 31) / kLanes;
