@@ -242,7 +242,10 @@ void launch_quant(const T* x, int64_t M, int64_t K, int64_t pad_rows, bool early
                   cudaStream_t st) {
   const int64_t chunks = fp4::k_tiles(FMT, K) * 4 * (fp4::Fmt<FMT>::kBlock / 16);
   const int64_t blocks = chunks <= 64 ? (pad_rows + 3) / 4 : pad_rows;
-  const dim3 grid((unsigned)(blocks < 148 * 64 ? blocks : 148 * 64));
+  // four to ten waves; an nvfp4 row's barriers like CTAs that go on to a next row (8192 x 4096
+  // 21.3 -> 18.4 us), mxfp4 rows do not (24576 x 4096 45.5 -> 46.6)
+  const int64_t cap = 148 * (FMT == FNI8_NVFP4 ? 24 : 64);
+  const dim3 grid((unsigned)(blocks < cap ? blocks : cap));
 #define FNI8_QUANT_FP4(G, KEEP)                                                                                     \
   launch_pdl(fp4::quant_rows<T, FMT, VW, G, KEEP>, grid, dim3(G < 128 ? 128 : G), 0, st, x, M, K, pad_rows, q, sf, rs, early)
   // few long rows: more threads to each (1 x 12288 nvfp4 2.9 us with 512, 7.7 with 128)
