@@ -195,34 +195,34 @@ __device__ void quant_rows(const T* __restrict__ src, int n, int K, int rank, in
   const uint4* rows = reinterpret_cast<const uint4*>(src);
   // Piece c of row i: this thread's pieces in turn, `per` to a row (zeros behind K), with the
   // loads of the next four in flight. (A queue, not an unrolled loop: short code.)
-  struct Pos {
-    int i, c;
-  };
-  auto settle = [&](Pos& p, int per) {
-    while (p.c >= per) {
-      p.c -= per;
-      p.i += peers;
-    }
-  };
   auto each = [&](int per, auto&& f) {
-    Pos at{rank, t0}, ahead{rank, t0};
+    const int di = threads / per * peers, dc = threads % per;
+    struct Pos {
+      int i, c;
+    };
+    auto advance = [&](Pos& p) {
+      p.i += di;
+      if ((p.c += dc) >= per) {
+        p.c -= per;
+        p.i += peers;
+      }
+    };
+    Pos at{rank + t0 / per * peers, t0 % per}, ahead = at;
     auto fetch = [&]() {
-      settle(ahead, per);
       uint4 u = make_uint4(0u, 0u, 0u, 0u);
       if (ahead.i < n && ahead.c < nc) u = rows[static_cast<int64_t>(ahead.i) * nc + ahead.c];
-      ahead.c += threads;
+      advance(ahead);
       return u;
     };
     uint4 q0 = fetch(), q1 = fetch(), q2 = fetch(), q3 = fetch();
 #pragma unroll 1
-    for (settle(at, per); at.i < n; settle(at, per)) {
+    for (; at.i < n; advance(at)) {
       const uint4 u = q0;
       q0 = q1;
       q1 = q2;
       q2 = q3;
       q3 = fetch();
       f(at.i, at.c, u);
-      at.c += threads;
     }
   };
   each(nc, [&](int i, int, const uint4& u) {
