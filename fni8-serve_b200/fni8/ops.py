@@ -409,7 +409,7 @@ def _fp4_shape(qt: QTensor, what: str) -> tuple[int, int]:
     Kp = qt.data.shape[-1] * 2
     K = Kp if qt.cols is None else int(qt.cols)
     rows = qt.data.numel() * 2 // Kp if Kp else 0
-    if qt.data.dtype != torch.uint8 or qt.data.dim() < 2 or K <= 0 or (K + 31) // 32 * 32 != Kp:
+    if qt.data.dtype != torch.uint8 or qt.data.dim() < 1 or K <= 0 or (K + 31) // 32 * 32 != Kp:
         raise ValueError(f"fni8.{what}: {qt.scheme} data {tuple(qt.data.shape)} {qt.data.dtype} does not pack "
                          f"{K} columns (two codes to a byte, rows padded to 32 values)")
     if qt.group_size not in (None, g):

@@ -42,6 +42,7 @@ from .moe import ExpertStack, combine, grouped_gemm, grouped_gemm_act, plan
 from .ops import (_ACT, _DT, _need_cuda, _stream, _vp, act_and_mul_quant, linear, linear_q_peer_cols,
                   quantize_rows)
 from .qtensor import QTensor
+from .quant import fp4
 
 
 def gather_rows(q: torch.Tensor, scale: torch.Tensor, slot_of_row: torch.Tensor, rows: int, top_k: int):
@@ -492,11 +493,15 @@ class ExpertParallelMoE:
 
 
 def shard_rows(qt: QTensor, world: int, rank: int) -> QTensor:
-    """Rows [r*N/P, (r+1)*N/P) of a per_row_i8 weight (output-channel shard)."""
+    """Rows [r*N/P, (r+1)*N/P) of a per_row_i8, mxfp4 or nvfp4 weight (output-channel shard)."""
     N = qt.data.shape[0]
     if N % world:
         raise ValueError(f"N={N} does not split over {world} ranks")
     lo, hi = rank * N // world, (rank + 1) * N // world
+    if qt.scheme in fp4.BLOCK:
+        rows = fp4.scale_rows(qt.scale, N, qt.scale.shape[1] * 4)[lo:hi]
+        return QTensor(qt.data[lo:hi].contiguous(), fp4.scale_tiles(rows), scheme=qt.scheme, group_size=qt.group_size,
+                       row_scale=None if qt.row_scale is None else qt.row_scale[lo:hi].contiguous(), cols=qt.cols)
     return QTensor(qt.data[lo:hi].contiguous(), qt.scale[lo:hi].contiguous(), scheme=qt.scheme)
 
 

@@ -115,8 +115,10 @@ def test_c_abi_refusals():
     assert need == 512 + 40 * 32 + 40 * 4
     assert linear(scratch=None) == n.ERR_WORKSPACE and linear(sb=need - 1) == n.ERR_WORKSPACE
     assert linear(scratch=bad) == n.ERR_ALIGN and linear(x=p + 1) == n.ERR_ALIGN
-    assert L.fni8_linear_fp4_scratch_bytes(n.NVFP4, 16, 8, 64) == 0  # one kernel
-    assert linear(M=16, x=bad, scratch=None, sb=0) == n.ERR_ALIGN
+    # one kernel, for what its threads hold in registers
+    assert L.fni8_linear_fp4_scratch_bytes(n.MXFP4, 16, 8, 64) == 0 and L.fni8_linear_fp4_scratch_bytes(n.NVFP4, 8, 8, 64) == 0
+    assert L.fni8_linear_fp4_scratch_bytes(n.NVFP4, 16, 8, 64) > 0
+    assert linear(M=8, x=bad, scratch=None, sb=0) == n.ERR_ALIGN
     assert L.fni8_linear_fp4_scratch_bytes(n.NVFP4, 16, 8, 63) > 0 and linear(M=16, K=63, sb=0) == n.ERR_WORKSPACE
     assert L.fni8_linear_fp4_scratch_bytes(9, 16, 8, 64) == 0 and L.fni8_linear_fp4_scratch_bytes(0, 0, 8, 64) == 0
     assert linear(M=0, x=None) == n.OK
@@ -154,3 +156,27 @@ def test_python_refusals():
         fni8.linear_fp4(ok, ok)
     with pytest.raises(RuntimeError):
         fni8.linear(x, ok)
+
+
+@pytest.mark.parametrize("scheme", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("N,world", [(256, 2), (260, 4), (9, 3)])
+def test_row_shards(scheme, N, world):
+    """An output-channel shard is the rows' own codes, scales and row scales, whatever tile they were in."""
+    import fni8
+    from fni8.parallel import shard_rows
+    from fni8.quant import fp4
+
+    codes, sf, row = O4.quantize(torch.randn(N, 200, generator=torch.Generator().manual_seed(N)).half(), scheme)
+    qt = fni8.QTensor(O4.pack(codes), fp4.scale_tiles(sf), scheme=scheme, group_size=fp4.BLOCK[scheme], row_scale=row,
+                      cols=200)
+    n = N // world
+    for r in range(world):
+        s = shard_rows(qt, world, r)
+        own = slice(r * n, (r + 1) * n)
+        assert s.scheme == scheme and s.group_size == qt.group_size and s.cols == 200
+        assert torch.equal(s.data, qt.data[own])
+        assert torch.equal(fp4.scale_rows(s.scale, n, sf.shape[1]), sf[own])
+        assert torch.equal(s.scale, fp4.scale_tiles(sf[own]))
+        assert s.row_scale is None if row is None else torch.equal(s.row_scale, row[own])
+    with pytest.raises(ValueError):
+        shard_rows(qt, 7, 0)

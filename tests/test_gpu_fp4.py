@@ -351,3 +351,31 @@ def test_weights_quantised_right_before(scheme, M):
         q = fni8.quantize_fp4(w, scheme)
         torch.cuda.synchronize()
         assert torch.equal(fni8.linear(x, q), y)
+
+
+@pytest.mark.parametrize("scheme", SCHEMES)
+@pytest.mark.parametrize("lead", [(), (2, 3), (0,), (4, 0)])
+def test_leading_dims(scheme, lead):
+    """Any leading dims, none at all among them: the values, codes and product of the flattened rows."""
+    import fni8
+
+    K, N = 70, 48
+    x = torch.randn(*lead, K, generator=gen(1)).half().to(DEV)
+    w = fni8.quantize_fp4(torch.randn(N, K, generator=gen(2)).half().to(DEV), scheme)
+    q, flat = fni8.quantize_fp4(x, scheme), fni8.quantize_fp4(x.reshape(-1, K), scheme)
+    assert fni8.dequantize_fp4(q).shape == x.shape
+    assert torch.equal(fni8.dequantize_fp4(q).reshape(-1, K), fni8.dequantize_fp4(flat))
+    for y in (fni8.linear(x, w), fni8.linear_fp4(q, w)):
+        assert y.shape == (*lead, N)
+        assert torch.equal(y.reshape(-1, N), fni8.linear_fp4(flat, w))
+
+
+@pytest.mark.parametrize("scheme", SCHEMES)
+def test_shards_give_the_columns(scheme):
+    import fni8
+    from fni8.parallel import shard_rows
+
+    x = torch.randn(40, 320, generator=gen(1)).half().to(DEV)
+    w = fni8.quantize_fp4(torch.randn(300, 320, generator=gen(2)).half().to(DEV), scheme)
+    y = torch.cat([fni8.linear(x, shard_rows(w, 3, r)) for r in range(3)], dim=1)
+    assert torch.equal(y, fni8.linear(x, w))
