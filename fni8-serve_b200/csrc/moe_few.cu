@@ -22,7 +22,7 @@
 //    no exchange. In few_down a CTA owns 16 output columns through all experts, keeps their
 //    int32 sums in shared memory and joins each token's k slots there: no atomics in global
 //    memory, no third kernel. With fewer experts than warps it splits their K.
-//  * Each CTA, or each cluster of eight where there are many values, routes, quantises the
+//  * Each CTA, or each cluster of four where there are many values, routes, quantises the
 //    rows and lists the experts for itself: cheaper than a launch that would hand them over.
 //    Where both kernels fit on an SM few_down does that too, and starts its weight loads, before
 //    it waits for few_gate_up; where they do not it reads the lists that few_gate_up leaves.
@@ -731,17 +731,18 @@ int few_stages(int cols, int rows, int64_t k_len, int slots, int E, int extra) {
   return 0;
 }
 
-// CTAs per cluster that share the preparation. Eight, where the rows have 16384 values in all:
-// sixteen tokens through 8 of 128 experts 64 us, 71 without clusters; fewer values are sooner
+// CTAs per cluster that share the preparation. Four, where the rows have 16384 values in all:
+// sixteen tokens through 8 of 128 experts 56 us, 66 in pairs, 61 in clusters of eight (which leave
+// 28 of the 148 SMs idle: 128 tiles of few_down then take two rounds); fewer values are sooner
 // quantised than shared (one token of 2048: 20.9 us, in clusters 21.1).
-int few_cluster(int64_t rows, int64_t k_len) { return rows * k_len >= 16384 ? 8 : 1; }
+int few_cluster(int64_t rows, int64_t k_len) { return rows * k_len >= 16384 ? 4 : 1; }
 
 // Grid of `want` CTAs at most, in clusters of cs that are resident at once.
 int few_grid(int64_t want, int smem, int cs) {
   const int sms = num_sms(current_device());
   int64_t n = want < sms ? want : sms;
   if (cs > 1) {
-    struct Entry { int dev, smem, n; };
+    struct Entry { int dev, smem, cs, n; };
     static Entry cache[64];
     static int used = 0;
     static std::mutex mu;
@@ -749,10 +750,10 @@ int few_grid(int64_t want, int smem, int cs) {
     const int dev = current_device();
     int most = -1;
     for (int i = 0; i < used; ++i)
-      if (cache[i].dev == dev && cache[i].smem == smem) most = cache[i].n;
+      if (cache[i].dev == dev && cache[i].smem == smem && cache[i].cs == cs) most = cache[i].n;
     if (most < 0) {
       most = max_active_clusters(few::kThreads, smem, cs);
-      if (most >= 0 && used < 64) cache[used++] = Entry{dev, smem, most};
+      if (most >= 0 && used < 64) cache[used++] = Entry{dev, smem, cs, most};
     }
     if (most < 1) most = sms / cs;
     n = (n + cs - 1) / cs;
