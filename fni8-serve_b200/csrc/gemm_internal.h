@@ -138,6 +138,8 @@ struct FewMoe {
   int32_t* t_ent_e;
   int32_t* t_ent_n;
   uint16_t* t_list;
+  int8_t* hq;  // [T k, I]
+  float* hs;   // [T k]
 };
 bool few_supported(int64_t T, int64_t H, int64_t k, int64_t E, int64_t I);
 int few_moe(const FewMoe& m, cudaStream_t st);

@@ -466,14 +466,14 @@ extern "C" size_t fni8_moe_experts_workspace_bytes(int64_t T, int64_t H, int64_t
   return moe_layout(T, H, top_k, E, I).total;
 }
 
-// Whether a call takes the two-kernel form. (Anything else, wrong arguments included, is for
+// Whether a call takes the few-token form (moe_few.cu). (Anything else, wrong arguments included, is for
 // the composed path below, whose results are the same.)
 static bool few_tokens(const void* x, int act, int64_t T, int64_t H, int64_t k, int64_t E, int64_t I) {
   return (act == FNI8_ACT_SILU || act == FNI8_ACT_GELU_TANH) && (reinterpret_cast<uintptr_t>(x) & 15u) == 0 &&
          few_supported(T, H, k, E, I);
 }
 
-// The two-kernel form's scratch within the composed path's workspace.
+// The few-token form's scratch within the composed path's workspace.
 static void few_scratch(FewMoe& m, uint8_t* b) {
   const MoeLayout L = moe_layout(m.T, m.H, m.k, m.E, m.I);
   m.h = b + L.h;
@@ -483,6 +483,8 @@ static void few_scratch(FewMoe& m, uint8_t* b) {
   m.t_ent_e = reinterpret_cast<int32_t*>(b + L.as);
   m.t_ent_n = reinterpret_cast<int32_t*>(b + L.hs);
   m.t_list = reinterpret_cast<uint16_t*>(b + L.y);  // 32 bytes per slot, of 2 H
+  m.hq = reinterpret_cast<int8_t*>(b + L.hq);
+  m.hs = reinterpret_cast<float*>(b + L.aq);  // 4 bytes per slot, of H
 }
 
 extern "C" int fni8_moe_experts_w8a8(const void* x, int dtype, int64_t T, int64_t H, const int32_t* topi,

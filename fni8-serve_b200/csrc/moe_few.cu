@@ -1,4 +1,4 @@
-// The routed-expert layer for a few tokens (T <= 16) in two kernels:
+// The routed-expert layer for a few tokens (T <= 16) in two kernels, or three:
 //
 //   few_gate_up  logits -> top-k (optional), int8 rows of x, then per active expert e and slot
 //                (t, j) routed to it   h[slot] = T(T(act(g)) u),
@@ -25,7 +25,9 @@
 //  * Each CTA, or each cluster of four where there are many values, routes, quantises the
 //    rows and lists the experts for itself: cheaper than a launch that would hand them over.
 //    Where both kernels fit on an SM few_down does that too, and starts its weight loads, before
-//    it waits for few_gate_up; where they do not it reads the lists that few_gate_up leaves.
+//    it waits for few_gate_up. Where they do not, it reads the lists that few_gate_up leaves, and
+//    h is quantised once by the row kernel of quant.cu, launched between the two (16 tokens
+//    through 8 of 128 experts 56 -> 51 us).
 //  * A CTA runs most of its code once, and an instruction line that is not in its SM's caches
 //    costs 0.1 us and more; so the preparation is short loops, not unrolled ones (listing the
 //    experts of one token: 4.9 us at first sight, 0.8 us the second time), and the weights pass
@@ -79,6 +81,9 @@ struct Layer {
   int32_t* t_ent_e;
   int32_t* t_ent_n;
   uint16_t* t_list;  // [T k][kEntry]
+  // not early: the int8 rows of h and their scales, quantised by a kernel between the two
+  const int8_t* hq;
+  const float* hs;
 };
 
 // Shared-memory plan of either kernel: `row` bytes of codes per row (odd multiple of 16 modulo
@@ -599,9 +604,25 @@ __global__ void __launch_bounds__(kThreads) few_down(const __grid_constant__ CUt
   int issued = min(steps, p.stages), consumed = 0;
   if (lane == 0)
     for (int i = 0; i < issued; ++i) issue();
-  pdl_wait();
-  quant_rows<T>(static_cast<const T*>(p.h), n, p.I, rank, peers, kThreads, codes, pl.row, h_s,
-                reinterpret_cast<uint32_t*>(smem + pl.top));
+  if (p.early) {
+    pdl_wait();
+    quant_rows<T>(static_cast<const T*>(p.h), n, p.I, rank, peers, kThreads, codes, pl.row, h_s,
+                  reinterpret_cast<uint32_t*>(smem + pl.top));
+  } else {
+    const int per = p.I >> 4, di = kThreads / per, dc = kThreads % per;
+    int c = threadIdx.x % per;
+#pragma unroll 1
+    for (int i = threadIdx.x / per; i < n; i += di) {
+      cp_async_16(codes + i * pl.row + c * 16, p.hq + static_cast<int64_t>(i) * p.I + c * 16);
+      if ((c += dc) >= per) {
+        c -= per;
+        ++i;
+      }
+    }
+    cp_async_commit();
+    for (int i = threadIdx.x; i < n; i += kThreads) h_s[i] = p.hs[i];
+    cp_async_wait_group<0>();
+  }
   join(peers);
   pdl_launch_dependents();
 
@@ -732,8 +753,8 @@ int few_stages(int cols, int rows, int64_t k_len, int slots, int E, int extra) {
 }
 
 // CTAs per cluster that share the preparation. Four, where the rows have 16384 values in all:
-// sixteen tokens through 8 of 128 experts 56 us, 66 in pairs, 61 in clusters of eight (which leave
-// 28 of the 148 SMs idle: 128 tiles of few_down then take two rounds); fewer values are sooner
+// 4 tokens of 8 large experts 59 us, 63 in pairs, 64 in clusters of eight, which leave 28 of the
+// 148 SMs idle; fewer values are sooner
 // quantised than shared (one token of 2048: 20.9 us, in clusters 21.1).
 int few_cluster(int64_t rows, int64_t k_len) { return rows * k_len >= 16384 ? 4 : 1; }
 
@@ -810,7 +831,7 @@ template <typename T, bool WIDE, int COLS>
 int launch_down(const few::Layer& p, const CUtensorMap& map, int smem, cudaStream_t st) {
   static std::atomic<bool> done[kMaxDevices] = {};
   if (int s = configure(few::few_down<T, WIDE, COLS>, done)) return s;
-  const int cs = few_cluster(p.T * p.k, p.I);
+  const int cs = p.early ? few_cluster(p.T * p.k, p.I) : 1;
   launch_cluster(few::few_down<T, WIDE, COLS>, few_grid(p.H / 16, smem, cs), cs, smem, st, map, p);
   return FNI8_OK;
 }
@@ -862,6 +883,11 @@ int launch_few(const few::Layer& layer, const FewPlan& f, int act, const CUtenso
   int s = act == FNI8_ACT_SILU ? gate_up_any<T, FNI8_ACT_SILU>(p, f, gu, st)
                                : gate_up_any<T, FNI8_ACT_GELU_TANH>(p, f, gu, st);
   if (s) return s;
+  if (!f.early) {
+    const int dtype = std::is_same<T, __half>::value ? FNI8_F16 : FNI8_BF16;
+    s = fni8_quantize_rows_i8(p.h, dtype, (int64_t)p.T * p.k, p.I, const_cast<int8_t*>(d.hq), const_cast<float*>(d.hs), st);
+    if (s) return s;
+  }
   if (d.I % 128 == 0)
     s = f.cols_d == 4 ? launch_down<T, true, 4>(d, dn, f.smem_d, st) : launch_down<T, true, 2>(d, dn, f.smem_d, st);
   else
@@ -903,7 +929,7 @@ int few_moe(const FewMoe& m, cudaStream_t st) {
   }
   few::Layer p{m.x, m.logits, m.topi, m.topw, m.sel_bias, (int)m.T, (int)m.H, (int)m.E, (int)m.I, (int)m.k, m.scoring,
                (int)m.n_groups, (int)m.topk_group, m.norm_topk, m.dtype, m.scaling, m.s_gu, m.s_dn, m.h, m.out, 0, 0, m.t_count, m.t_slot_e, m.t_slot_w, m.t_ent_e,
-               m.t_ent_n, m.t_list};
+               m.t_ent_n, m.t_list, m.hq, m.hs};
   return m.dtype == FNI8_F16 ? launch_few<__half>(p, f, m.act, gu, dn, st)
                               : launch_few<__nv_bfloat16>(p, f, m.act, gu, dn, st);
 }

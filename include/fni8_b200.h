@@ -369,7 +369,7 @@ FNI8_API int fni8_moe_experts_w8a8(const void* x, int dtype, int64_t T, int64_t 
 /* The same from the router's logits [T, E] on: fni8_moe_route (weights rounded to dtype), then
  * fni8_moe_experts_w8a8 (SparseMoE.forward without the shared expert,
  * fni8serve/models/moe.py:62-105); the routing is not returned. Up to 16 tokens, where the
- * rows fit into shared memory, run in two kernels that read each active expert's weights
+ * rows fit into shared memory, run in two or three kernels that read each active expert's weights
  * once (fni8_moe_experts_w8a8 likewise); the results are those of the separate calls, bit for
  * bit, for any T. E <= 512. */
 FNI8_API size_t fni8_moe_layer_workspace_bytes(int64_t T, int64_t H, int64_t top_k, int64_t E, int64_t I);
