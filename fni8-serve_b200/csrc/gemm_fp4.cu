@@ -11,16 +11,18 @@
 // and BN rows of w with the 128-byte swizzle, plus their scale tiles as they lie in memory
 // (512 bytes each, no swizzle); tcgen05.cp brings those into tensor memory.
 //
-// What bounds it: as the int8 kernel, the feed of shared memory from L2 (about 45 B/clk of an
-// SM). The copies must not come on top of that. Measured on B200: one thread issues one in 45
-// cycles, whatever its shape, so the 12 of an nvfp4 stage of 256 columns take 540, its MMAs
-// 512; issued by the MMAs' thread they overlap neither the MMAs before its last commit nor
-// those behind them (8192 x 4096 x 16384: mxfp4 256 us, nvfp4 358, without the copies 183 and
-// 189). From other threads they leave the MMAs at 514 cycles a stage, but a stage's copies then
-// complete some 1400 cycles after their issue. So two more warps issue them (211 and 274 us
-// with one, 209 and 232 with two, 219 and 236 with three), and the scales run ahead: their
-// ring is kLead stages deeper than the operands', their tiles are loaded before the operands
-// of earlier stages, and SETS sets of tensor-memory columns take turns.
+// What bounds it (8192 rows): a stage of a pair takes some 835 cycles where its MMAs take 512, and
+// a tile 2350 more (K = 4096: 350 us, tensor pipe busy half the time, L2 a third; K = 12288: 160).
+// Neither the bytes of the feed (256 x 384 tiles, a sixth fewer, took 347 and 169 us) nor the
+// power (operands of zeros 347 and 150) holds it there, the scale copies do in part. Measured on
+// B200: one thread issues one in 45 cycles, whatever its shape, so the 12 of an nvfp4 stage of 256
+// columns take 540; issued by the MMAs' thread they overlap neither the MMAs before its last
+// commit nor those behind them (8192 x 4096 x 16384: mxfp4 256 us, nvfp4 358, without the copies
+// 183 and 189). From other threads they leave the MMAs alone, but a stage's copies then complete
+// some 1400 cycles after their issue. So two more warps issue them (211 and 274 us with one, 209
+// and 232 with two, 219 and 236 with three), and the scales run ahead: their ring is kLead stages
+// deeper than the operands', their tiles are loaded before the operands of earlier stages, and
+// SETS sets of tensor-memory columns take turns.
 #include "fp4_common.cuh"
 #include "gemm_internal.h"
 

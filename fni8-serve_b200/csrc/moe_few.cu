@@ -855,7 +855,8 @@ bool few_plan(int64_t T, int64_t H, int64_t k, int64_t E, int64_t I, FewPlan* p)
     return p->stages_d > 0;
   };
   // Both kernels on an SM where they fit and the weights are few: one token through 8 of 128
-  // experts (38 MB) 21 us, 23 with wide stages; through 2 of 4096 x 4096 (101 MB) 41 and 38.6.
+  // experts (38 MB) 21.7 us, 24 with wide stages; through 2 of 4096 x 4096 (101 MB) 32 and 34, two
+  // tokens (201 MB) 57 and 48.
   p->early = 0;
   if ((int64_t)n * 3 * H * I <= (128 << 20) && gate_up(2) && down(2) && p->smem_g + p->smem_d + 2 * 2048 <= kSmemMax) {
     p->early = 1;
