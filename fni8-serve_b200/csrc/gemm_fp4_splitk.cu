@@ -5,8 +5,8 @@
 //
 // Bound: HBM, N K (1/2 + 1/g) bytes of weights read once. As in gemm_splitk.cu the operands
 // are swapped (128 weight rows = MMA M, NT tokens = MMA N) and a cluster of S CTAs splits the
-// K range of a weight tile (and of a block of 128 tokens, where there are more), S chosen so that the grid fills the GPU once; weights are loaded
-// before the wait for the quantiser. Here the S partial accumulators meet in shared memory:
+// K range of a weight tile (and of a block of 128 tokens, where there are more), S chosen so that the grid fills the GPU
+// once; the first weights enter L2 while the kernel in front still runs. Here the S partial accumulators meet in shared memory:
 // CTA r owns a share of the token columns, every CTA stores the columns of the others into
 // their landing areas (distributed shared memory, 16-byte pieces of four tokens, the weight row
 // innermost), and the owner adds the S parts in rank order, so the result does not depend on
@@ -181,6 +181,22 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int kbeg = static_cast<int>(static_cast<int64_t>(rank) * kb / S);
   const int nk = static_cast<int>(static_cast<int64_t>(rank + 1) * kb / S) - kbeg;
 
+  // The kernel in front may be the one that writes the weights or their scales, and what a grid wrote is
+  // promised to be seen only behind the wait; so ahead of it the first ring's weights only enter L2, where
+  // a line that is written later stays right.
+  const int pre = nk < stages ? nk : stages;
+  if (warp == 2 && lane == 0) {
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmSW);
+    if constexpr (!FUSED) {
+      tma_prefetch_desc(&tmX);
+      tma_prefetch_desc(&tmSX);
+    }
+    for (int i = 0; i < pre; ++i) {
+      tma_prefetch_l2_2d(&tmW, (kbeg + i) * 128, tile * 128);
+      tma_prefetch_l2_2d(&tmSW, 0, (tile * ktiles + (kbeg + i) * C::TILES) * 4);
+    }
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
@@ -202,6 +218,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t tmem_base = *tmem_slot;
   // the peers have started before anything is stored into their shared memory
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  pdl_wait();  // of every thread, before any operand is read
 
   int okt = 0;
   float rw = 1.0f, bias = 0.0f;  // of this epilogue thread's weight row
@@ -210,12 +227,6 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0) {
-      tma_prefetch_desc(&tmW);
-      tma_prefetch_desc(&tmSW);
-      if constexpr (!FUSED) {
-        tma_prefetch_desc(&tmX);
-        tma_prefetch_desc(&tmSX);
-      }
       auto load_w = [&](int s, int k) {
         uint8_t* dst = smem + s * C::STAGE;
         mbar_arrive_expect_tx(&full[s], C::STAGE);
@@ -229,10 +240,10 @@ __global__ void __launch_bounds__(kThreads, 2)
           tma_load_2d(&tmX, &full[s], dst + C::SF_BYTES, k * 128, m0);
         }
       };
-      const int pre = nk < stages ? nk : stages;
-      for (int i = 0; i < pre; ++i) load_w(i, kbeg + i);
-      pdl_wait();
-      for (int i = 0; i < pre; ++i) load_x(i, kbeg + i);
+      for (int i = 0; i < pre; ++i) {
+        load_w(i, kbeg + i);
+        load_x(i, kbeg + i);
+      }
       int stage = pre % stages, issued = pre;
       uint32_t ph = pre == stages ? 1u : 0u, armed = 0;
       for (int i = pre; i < nk; ++i) {
@@ -285,7 +296,6 @@ __global__ void __launch_bounds__(kThreads, 2)
   } else {
     if constexpr (FMT == FNI8_NVFP4)
       if (n < N) rw = __ldg(epi.w_rs + n);
-    pdl_wait();
     if (n < N && epi.bias != nullptr)
       bias = epi.bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(epi.bias)[n])
                       : __half2float(static_cast<const __half*>(epi.bias)[n]);

@@ -1,0 +1,93 @@
+"""fni8.linear right behind the kernels that write its weight: nothing of it may be read before they have ended."""
+import pytest
+import torch
+
+pytestmark = [pytest.mark.gpu,
+              pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a B200")]
+
+DEV = "cuda"
+SCHEMES = ["mxfp4", "nvfp4"]
+# one kernel that quantises x, split-K behind the quantiser (32, 64 and 128 tokens to a block), tiles
+ROWS = [1, 16, 17, 64, 128, 300]
+
+
+def weights(n, N, K, scheme):
+    import fni8
+
+    g = torch.Generator(device=DEV).manual_seed(K)
+    out = []
+    for i in range(n):
+        w = fni8.quantize_fp4((0.05 * (i + 1) * torch.randn(N, K, generator=g, device=DEV)).half(), scheme)
+        if w.row_scale is not None:
+            w.row_scale.mul_(1.0 + 0.37 * i)
+        out.append(w)
+    return out
+
+
+def into(dst, src):
+    """The weight src into dst's tensors: one small kernel to each part, the row scale last."""
+    dst.data.copy_(src.data)
+    dst.scale.copy_(src.scale)
+    if dst.row_scale is not None:
+        dst.row_scale.copy_(src.row_scale)
+
+
+@pytest.mark.parametrize("scheme", SCHEMES)
+@pytest.mark.parametrize("M", ROWS)
+def test_weight_rewritten_in_place(scheme, M):
+    import fni8
+
+    N, K = 2304, 4096
+    x = torch.randn(M, K, generator=torch.Generator(device=DEV).manual_seed(M), device=DEV).half()
+    xq = fni8.quantize_fp4(x, scheme)
+    bias = torch.zeros(N, device=DEV).half()
+    src = weights(4, N, K, scheme)
+    live = weights(1, N, K, scheme)[0]
+    want = [fni8.linear(x, w, bias=bias + i) for i, w in enumerate(src)]
+    torch.cuda.synchronize()
+    got, got_q, order = [], [], [0, 3, 1, 2, 3, 0, 2, 1]
+    for i in order:
+        into(live, src[i])
+        bias.fill_(i)
+        got.append(fni8.linear(x, live, bias=bias))
+        into(live, src[3 - i])
+        bias.fill_(3 - i)
+        got_q.append(fni8.linear_fp4(xq, live, bias=bias))
+    torch.cuda.synchronize()
+    for i, y, yq in zip(order, got, got_q):
+        assert torch.equal(y, want[i]) and torch.equal(yq, want[3 - i])
+    # only the row scale changes, right in front of the call
+    if scheme == "nvfp4":
+        ys = []
+        for f in (2.0, 0.5, 4.0, 0.25):
+            live.row_scale.mul_(f)
+            ys.append(fni8.linear(x, live))
+        torch.cuda.synchronize()
+        for y, f in zip(ys, (1.0, 0.5, 2.0, 0.5)):
+            ref = fni8.QTensor(live.data, live.scale, scheme=scheme, row_scale=live.row_scale * (2.0 * f), cols=K)
+            torch.cuda.synchronize()
+            assert torch.equal(y, fni8.linear(x, ref))
+    assert fni8.device_status() == 0
+
+
+@pytest.mark.parametrize("scheme", SCHEMES)
+@pytest.mark.parametrize("M", ROWS)
+def test_weight_rewritten_within_a_graph(scheme, M):
+    import fni8
+
+    N, K = 1152, 2048
+    x = torch.randn(M, K, generator=torch.Generator(device=DEV).manual_seed(M), device=DEV).half()
+    src = weights(2, N, K, scheme)
+    live = weights(1, N, K, scheme)[0]
+    want = [fni8.linear(x, w) for w in src]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ys = []
+        for i in (0, 1, 0, 1):
+            into(live, src[i])
+            ys.append(fni8.linear(x, live))
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, want[i]) for y, i in zip(ys, (0, 1, 0, 1)))
