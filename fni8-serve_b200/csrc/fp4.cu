@@ -55,8 +55,8 @@ __device__ __forceinline__ uint32_t raw_max(const Raw16& r) {
 
 // GROUP threads per row. KEEP: chunks of a row that each thread holds in registers (0: the
 // row is read a second time, for longer ones). Rows [M, pad_rows) only get zero scales. early:
-// the next kernel may start at once. It must not where the rows may be weights: the GEMMs load
-// those before they wait for the kernel in front of them.
+// the next kernel may start at once, where that is the GEMM of these rows, which sets itself up meanwhile.
+// Other kernels only take room from this one (1024 x 12288 mxfp4 back to back 7.7 us, with it 10.1).
 template <typename T, int FMT, int VW, int GROUP, int KEEP>
 __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP) quant_rows(const T* __restrict__ x, int64_t M, int64_t K,
                                                                         int64_t pad_rows, uint8_t* __restrict__ q,

@@ -96,8 +96,8 @@ struct Fp4Gemm {
 };
 int fp4_check_rows(const void* x, int dtype, int format, int64_t M, int64_t K, const uint8_t* q, const uint8_t* sf,
                    const float* row_scale);
-// pad: the rows may be weights. The scales of the rows behind M in the last tile are zeroed, and
-// the next kernel starts when this one has ended (the GEMMs load weights before they wait).
+// pad: the scales of the rows behind M in the last tile are zeroed, and the next kernel starts when this one
+// has ended; else (the rows of a GEMM that follows at once) it may start early.
 int fp4_quantize(const void* x, int dtype, int format, int64_t M, int64_t K, bool pad, uint8_t* q, uint8_t* sf,
                  float* row_scale, cudaStream_t st);
 // The swap-AB split-K kernel (gemm_fp4_splitk.cu), and into how many parts it would cut K at M > 64.
