@@ -17,8 +17,6 @@
 // the weights are on their way; the ring then holds weights only. It saves the quantiser's
 // launch (2.5 us at 4096 values, 5 at 12288 of the pair's 9 and 14). An nvfp4 row's maximum
 // goes through the cluster's shared memory: each CTA posts its slice's.
-#include <mutex>
-
 #include "fp4_common.cuh"
 #include "gemm_internal.h"
 
@@ -416,21 +414,6 @@ namespace {
 
 constexpr int kMinRing = 2;
 
-// Clusters of S CTAs with `smem` bytes that are resident at once, remembered per device.
-int resident_clusters(int smem, int S) {
-  struct Entry { int dev, smem, S, n; };
-  static Entry cache[64];
-  static int used = 0;
-  static std::mutex mu;
-  std::lock_guard<std::mutex> lock(mu);
-  const int dev = current_device();
-  for (int i = 0; i < used; ++i)
-    if (cache[i].dev == dev && cache[i].smem == smem && cache[i].S == S) return cache[i].n;
-  const int n = max_active_clusters(fp4s::kThreads, smem, S);
-  if (n >= 0 && used < 64) cache[used++] = Entry{dev, smem, S, n};
-  return n;
-}
-
 struct Plan {
   int S, stages, xstages, smem;
   bool fits;
@@ -466,7 +449,7 @@ Plan plan_splitk(int64_t rows, int64_t N, int64_t K) {
   most = most < 1 ? 1 : most > 8 ? 8 : most;
   Plan p = plan((int)(most > kb ? kb : most));
   while (p.S > 1) {
-    const int n = p.fits ? resident_clusters(p.smem, p.S) : -1;
+    const int n = p.fits ? max_active_clusters(fp4s::kThreads, p.smem, p.S) : -1;
     if (p.fits && (n < 0 || tiles <= (!FUSED && NT <= 32 ? n - n / 8 : n))) break;
     p = plan(p.S - 1);
   }

@@ -26,10 +26,11 @@
 //    are published; its weight loads then queue behind this kernel's.
 // Shared memory stays under half an SM up to NT = 128, so two CTAs (or this kernel and
 // the next) share an SM. Every mbarrier wait is bounded (fni8_common.cuh).
-#include <mutex>
+#include <tuple>
 
 #include "fni8_common.cuh"
 #include "gemm_internal.h"
+#include "size_memo.h"
 
 #include <stdio.h>
 #include <stdlib.h>
@@ -483,14 +484,8 @@ static cudaError_t configure_splitk(int dev) {
 // shared-memory size, while two of its CTAs measurably run on one SM together.)
 static __global__ void __launch_bounds__(1024, 1) occupancy_standin() {}
 
-// How many S-CTA clusters of `threads`-thread CTAs with `smem` bytes of shared memory can
-// be resident at once (clusters live inside one GPC, so this is below SMs x CTAs-per-SM /
-// S). Registers are not modelled (the callers' kernels fit two CTAs per SM by registers).
-// -1 when the runtime cannot tell (no device).
-int max_active_clusters(int threads, int smem, int S) {
+static int query_active_clusters(int dev, int threads, int smem, int S) {
   static std::atomic<bool> configured[kMaxDevices] = {};
-  const int dev = current_device();
-  if (dev < 0 || dev >= kMaxDevices) return -1;
   if (!configured[dev]) {
     if (cudaFuncSetAttribute(occupancy_standin, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024) !=
         cudaSuccess) {
@@ -518,19 +513,21 @@ int max_active_clusters(int threads, int smem, int S) {
   return n;
 }
 
-static int max_clusters(int nt, int smem, int S) {
-  (void)nt;  // the ring size (smem) carries the token count's effect
-  struct Entry { int dev, smem, S, n; };
-  static Entry cache[64];
-  static int used = 0;
-  static std::mutex mu;  // GEMMs may be planned from several host threads
-  std::lock_guard<std::mutex> lock(mu);
+// How many S-CTA clusters of `threads`-thread CTAs with `smem` bytes of shared memory can
+// be resident at once (clusters live inside one GPC, so this is below SMs x CTAs-per-SM /
+// S). Registers are not modelled (the callers' kernels fit two CTAs per SM by registers).
+// -1 when the runtime cannot tell (no device). Asked once for a size, then looked up.
+int max_active_clusters(int threads, int smem, int S) {
+  struct Key {
+    int dev, threads, smem, S;
+    bool operator<(const Key& o) const {
+      return std::tie(dev, threads, smem, S) < std::tie(o.dev, o.threads, o.smem, o.S);
+    }
+  };
+  static SizeMemo<Key> memo;
   const int dev = current_device();
-  for (int i = 0; i < used; ++i)
-    if (cache[i].dev == dev && cache[i].smem == smem && cache[i].S == S) return cache[i].n;
-  const int n = max_active_clusters(splitk::kThreads, smem, S);
-  if (n >= 0 && used < 64) cache[used++] = Entry{dev, smem, S, n};
-  return n;
+  if (dev < 0 || dev >= kMaxDevices) return -1;
+  return memo.get(Key{dev, threads, smem, S}, [&] { return query_active_clusters(dev, threads, smem, S); });
 }
 
 // NT: tokens rounded up to a power of two >= 16. S: the cluster size that brings the grid
@@ -583,7 +580,7 @@ static bool plan_splitk(int64_t M, int64_t N, int64_t K, SplitPlan* p) {
   if (S > kb) S = kb;
   if (!plan_ring(nt, S, p)) return false;
   while (forced_s < 1 && S > 1) {
-    const int mc = max_clusters(nt, p->smem, S);
+    const int mc = max_active_clusters(splitk::kThreads, p->smem, S);
     if (mc < 0 || n_tiles <= mc) break;
     --S;
     if (!plan_ring(nt, S, p)) return false;
@@ -593,7 +590,8 @@ static bool plan_splitk(int64_t M, int64_t N, int64_t K, SplitPlan* p) {
   p->ws_bytes = S > 1 ? static_cast<size_t>(p->grid) * nt * splitk::BNW * 4 : 0;
   if (FNI8_TUNE_PLAN_LOG)
     fprintf(stderr, "fni8 split-K plan M=%lld N=%lld K=%lld: NT=%d S=%d grid=%d stages=%d smem=%d resident clusters=%d\n",
-            (long long)M, (long long)N, (long long)K, nt, S, p->grid, p->stages, p->smem, max_clusters(nt, p->smem, S));
+            (long long)M, (long long)N, (long long)K, nt, S, p->grid, p->stages, p->smem,
+            max_active_clusters(splitk::kThreads, p->smem, S));
   return true;
 }
 
@@ -627,7 +625,7 @@ static int launch_splitk(const CUtensorMap& tw, const CUtensorMap& tx, const spl
 bool splitk_split_one_wave(int64_t M, int64_t N, int64_t K) {
   SplitPlan p;
   if (N >= (1LL << 31) || K >= (1LL << 31) || !plan_splitk(M, N, K, &p) || p.S < 2) return false;
-  const int mc = max_clusters(p.nt, p.smem, p.S);
+  const int mc = max_active_clusters(splitk::kThreads, p.smem, p.S);
   return mc >= 0 && p.grid / p.S <= mc;
 }
 

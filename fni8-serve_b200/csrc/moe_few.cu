@@ -35,7 +35,6 @@
 //  * Lane (g, q) of a warp reads the 16-byte pieces 2 q + j (j = 0, 1) of row g of a 128-byte
 //    column: with the swizzle, eight neighbouring lanes then touch all 32 banks. The order of
 //    K inside a piece is the same on both sides of the product, so it needs no shuffle.
-#include <mutex>
 #include <type_traits>
 
 #include "fni8_common.cuh"
@@ -763,19 +762,7 @@ int few_grid(int64_t want, int smem, int cs) {
   const int sms = num_sms(current_device());
   int64_t n = want < sms ? want : sms;
   if (cs > 1) {
-    struct Entry { int dev, smem, cs, n; };
-    static Entry cache[64];
-    static int used = 0;
-    static std::mutex mu;
-    std::lock_guard<std::mutex> lock(mu);
-    const int dev = current_device();
-    int most = -1;
-    for (int i = 0; i < used; ++i)
-      if (cache[i].dev == dev && cache[i].smem == smem && cache[i].cs == cs) most = cache[i].n;
-    if (most < 0) {
-      most = max_active_clusters(few::kThreads, smem, cs);
-      if (most >= 0 && used < 64) cache[used++] = Entry{dev, smem, cs, most};
-    }
+    int most = max_active_clusters(few::kThreads, smem, cs);
     if (most < 1) most = sms / cs;
     n = (n + cs - 1) / cs;
     n = (n < most ? n : most) * cs;
