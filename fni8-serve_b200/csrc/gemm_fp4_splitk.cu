@@ -53,6 +53,10 @@ struct Cfg {
   static constexpr int SF_COLS = 8 * TILES;  // weights', then tokens' scales of a stage
   static constexpr int COLS = ACC_COLS + 2 * SF_COLS;
   static constexpr int TMEM_COLS = COLS <= 64 ? 64 : COLS <= 128 ? 128 : 256;
+  // A CTA holds its columns while it waits for its cluster, and another's allocation waits for columns: clusters of
+  // two streams could wait for each other for good. So no CTA takes a larger share of an SM's 512 columns than of
+  // its 228 KB of shared memory (1 KB of them the system's, for each CTA): what is resident together always fits.
+  static constexpr int MIN_SMEM = TMEM_COLS * (228 * 1024 / 512) - 1024;
   static_assert(STAGE % 1024 == 0, "stages keep the 1024-byte alignment of the swizzle");
 };
 
@@ -438,7 +442,8 @@ Plan plan_splitk(int64_t rows, int64_t N, int64_t K) {
     n = n < fp4s::kMaxStages ? n : fp4s::kMaxStages;
     n = n < per ? n : per;
     const bool slice = !FUSED || M * per * 32 <= 128 * fp4s::fused_chunks(FMT);
-    return Plan{S, (int)n, per, (int)(fixed + n * C::STAGE), slice && n >= (per < kMinRing ? per : kMinRing)};
+    const int64_t smem = fixed + n * C::STAGE;
+    return Plan{S, (int)n, per, (int)(smem < C::MIN_SMEM ? C::MIN_SMEM : smem), slice && n >= (per < kMinRing ? per : kMinRing)};
   };
   if constexpr (NT == 16 && !FUSED) {
     // split as the fused form does, so that both give the same sums

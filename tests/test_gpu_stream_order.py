@@ -91,3 +91,26 @@ def test_weight_rewritten_within_a_graph(scheme, M):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(y, want[i]) for y, i in zip(ys, (0, 1, 0, 1)))
+
+
+@pytest.mark.parametrize("scheme", SCHEMES)
+def test_clusters_of_two_streams(scheme):
+    """Split-K clusters of every width at once on three streams, short K among them (small CTAs, many to an SM): each
+    result is that of the call alone."""
+    import fni8
+
+    sizes = [(128, 1536, 4096), (17, 9216, 512), (64, 6144, 768), (16, 12288, 512), (66, 2048, 5120), (20, 4096, 512)]
+    g = torch.Generator(device=DEV).manual_seed(1)
+    ws = [fni8.quantize_fp4((0.05 * torch.randn(N, K, generator=g, device=DEV)).half(), scheme) for _, N, K in sizes]
+    xs = [torch.randn(M, K, generator=g, device=DEV).half() for M, _, K in sizes]
+    want = [fni8.linear(x, w) for x, w in zip(xs, ws)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for r in range(40):
+        for i in range(len(sizes)):
+            with torch.cuda.stream(streams[(i + r) % 3]):
+                got.append((i, fni8.linear(xs[i], ws[i])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i, y in got)
+    assert fni8.device_status() == 0
