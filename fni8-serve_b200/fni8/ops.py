@@ -411,7 +411,7 @@ def _fp4_shape(qt: QTensor, what: str) -> tuple[int, int]:
     rows = qt.data.numel() * 2 // Kp if Kp else 0
     if qt.data.dtype != torch.uint8 or qt.data.dim() < 1 or K <= 0 or (K + 31) // 32 * 32 != Kp:
         raise ValueError(f"fni8.{what}: {qt.scheme} data {tuple(qt.data.shape)} {qt.data.dtype} does not pack "
-                         f"{K} columns (two codes to a byte, rows padded to 32 values)")
+                         f"{K} columns (two codes to a byte, rows padded to 32 values: fni8.quant.fp4.pad_codes)")
     if qt.group_size not in (None, g):
         raise ValueError(f"fni8.{what}: {qt.scheme} has blocks of {g} values (group_size {qt.group_size})")
     sc = qt.scale
