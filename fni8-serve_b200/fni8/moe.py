@@ -18,8 +18,9 @@ pipeline without host synchronisation (capturable in a CUDA graph):
 (moe.py:25-60), so `fni8serve.models.moe.SparseMoE = fni8.moe.SparseMoE` (or the
 one-line import swap in that file) moves every MoE family onto the grouped kernels.
 
-`layer` is that pipeline in one call. Up to 16 tokens (a decode step) it runs in two or three
-kernels that stream each active expert's weights once, with the same results bit for bit.
+`layer` is that pipeline in one call. Up to 16 tokens (a decode step), where their int8 rows fit
+into shared memory, it runs in two or three kernels that stream each active expert's weights
+once, with the same results bit for bit.
 """
 from __future__ import annotations
 
@@ -189,7 +190,8 @@ def layer(x: torch.Tensor, logits: torch.Tensor, stack: ExpertStack, top_k: int,
           sel_bias: torch.Tensor | None = None, num_expert_groups: int | None = None, topk_group: int | None = None,
           norm_topk_prob: bool = True, scaling: float = 1.0, act: str = "silu") -> torch.Tensor:
     """The routed layer from the router's logits on: experts(x, *route(logits, ...), stack), bit
-    for bit, in one native call; up to 16 tokens in two or three kernels (moe_few.cu). x [T, H],
+    for bit, in one native call; up to 16 tokens in two or three kernels (moe_few.cu), as long as
+    T k (I + 150) and T H are below some 160,000. x [T, H],
     logits [T, E]; the other arguments as in `route` (weights are rounded to x.dtype)."""
     _need_cuda(x, "moe.layer")
     if act not in _ACT:

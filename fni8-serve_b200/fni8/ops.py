@@ -457,8 +457,9 @@ def quantize_fp4(x: torch.Tensor, scheme: str = "mxfp4") -> QTensor:
 
 
 def dequantize_fp4(qt: QTensor, dtype: torch.dtype = torch.float16) -> torch.Tensor:
-    """The values [..., K] of an mxfp4 or nvfp4 QTensor, rounded once to dtype (float16,
-    bfloat16 or float32)."""
+    """The values [..., K] of an mxfp4 or nvfp4 QTensor in dtype (float16, bfloat16 or float32).
+    code * scale is exact; its product with a row scale is rounded to fp32 (exact for powers of
+    two, which quantize_fp4 writes), then to dtype."""
     _need_cuda(qt.data, "dequantize_fp4")
     M, K = _fp4_shape(qt, "dequantize_fp4")
     odt = {torch.float16: nat.F16, torch.bfloat16: nat.BF16, torch.float32: nat.F32}.get(dtype)
@@ -493,7 +494,9 @@ def _fp4_bias(bias: torch.Tensor | None, N: int, dtype: torch.dtype, dev: torch.
 def linear_fp4(xq: QTensor, qt: QTensor, bias: torch.Tensor | None = None,
                out_dtype: torch.dtype = torch.float16) -> torch.Tensor:
     """y[..., N] = xq . qt^T (+ bias) for activations and a weight quantised by quantize_fp4
-    to the same scheme: summed in fp32 by the block-scaled tensor core, rounded once."""
+    to the same scheme: summed in fp32 by the block-scaled tensor core, then times both row scales
+    (+ bias) in fp32, then rounded to out_dtype. The order of the sum depends on the number of
+    rows, so a row alone and in a batch may differ in the last bits (int8 weights do not)."""
     _need_cuda(xq.data, "linear_fp4")
     if xq.scheme != qt.scheme:
         raise ValueError(f"fni8.linear_fp4: activations {xq.scheme}, weight {qt.scheme}")

@@ -260,13 +260,17 @@ FNI8_API size_t fni8_fp4_scale_bytes(int format, int64_t M, int64_t K);
  * or a NaN gets the scale NaN, and does not enter its row's maximum. Any K. */
 FNI8_API int fni8_quantize_rows_fp4(const void* x, int dtype, int format, int64_t M, int64_t K, uint8_t* q,
                                     uint8_t* sf, float* row_scale, void* stream);
-/* The values of a quantised matrix, rounded once to out_dtype (F16, BF16 or F32): out[M, K]. */
+/* The values of a quantised matrix in out_dtype (F16, BF16 or F32), out[M, K]: code * sf is exact, its product with
+ * row_scale is rounded to fp32 (exact for the powers of two that the quantiser writes), then to out_dtype. */
 FNI8_API int fni8_dequantize_rows_fp4(const uint8_t* q, const uint8_t* sf, const float* row_scale, int format,
                                       int64_t M, int64_t K, void* out, int out_dtype, void* stream);
 
 /* out[M, N] = a . w^T for quantised a[M, K] and w[N, K] of one format: the block-scaled sum
- * in fp32, then (sum * a_row_scale[m]) * w_row_scale[n] (+ bias[n]), rounded once to
- * out_dtype (F16 or BF16; bias in out_dtype or NULL). q rows 16-byte aligned. No workspace:
+ * in fp32, then (sum * a_row_scale[m]) * w_row_scale[n] (+ bias[n]), each step rounded to fp32,
+ * and the result to out_dtype (F16 or BF16; bias in out_dtype or NULL). K is cut into parts by
+ * M, N and K, so the order of a row's fp32 sum depends on M: the same for every call of the same
+ * sizes, but a row alone and in a batch may differ in the last bits. Operands are read behind
+ * griddepcontrol.wait: the kernel in front may be the one that writes them. q rows 16-byte aligned. No workspace:
  * concurrent calls are independent. */
 FNI8_API int fni8_gemm_fp4(const uint8_t* a, const uint8_t* a_sf, const float* a_row_scale, const uint8_t* w,
                            const uint8_t* w_sf, const float* w_row_scale, const void* bias, void* out, int out_dtype,
@@ -369,7 +373,7 @@ FNI8_API int fni8_moe_experts_w8a8(const void* x, int dtype, int64_t T, int64_t 
 /* The same from the router's logits [T, E] on: fni8_moe_route (weights rounded to dtype), then
  * fni8_moe_experts_w8a8 (SparseMoE.forward without the shared expert,
  * fni8serve/models/moe.py:62-105); the routing is not returned. Up to 16 tokens, where the
- * rows fit into shared memory, run in two or three kernels that read each active expert's weights
+ * int8 rows fit into shared memory (about T top_k (I + 150) and T H up to 160,000), run in two or three kernels that read each active expert's weights
  * once (fni8_moe_experts_w8a8 likewise); the results are those of the separate calls, bit for
  * bit, for any T. E <= 512. */
 FNI8_API size_t fni8_moe_layer_workspace_bytes(int64_t T, int64_t H, int64_t top_k, int64_t E, int64_t I);
