@@ -12,7 +12,8 @@
 // (512 bytes each, no swizzle); tcgen05.cp brings those into tensor memory.
 //
 // What bounds it (8192 rows): a stage of a pair takes some 835 cycles where its MMAs take 512, and
-// a tile 2350 more (K = 4096: 350 us, tensor pipe busy half the time, L2 a third; K = 12288: 160).
+// a tile 2350 more (K = 4096: 350 us at the full clock, 370 to 430 in long runs under the power cap;
+// tensor pipe busy half the time, L2 a third; K = 12288: 160).
 // Neither the bytes of the feed (256 x 384 tiles, a sixth fewer, took 347 and 169 us) nor the
 // power (operands of zeros 347 and 150) holds it there, the scale copies do in part. Measured on
 // B200: one thread issues one in 45 cycles, whatever its shape, so the 12 of an nvfp4 stage of 256

@@ -15,7 +15,7 @@
 // FUSED (fni8_linear_fp4, up to 16 tokens): the epilogue warps quantise the CTA's K slice of
 // the 16-bit rows themselves, straight into the swizzled operand tiles and scale tiles, while
 // the weights are on their way; the ring then holds weights only. It saves the quantiser's
-// launch (2.5 us at 4096 values, 5 at 12288 of the pair's 9 and 14). An nvfp4 row's maximum
+// launch and its scratch, and up to 1.6 us on the device (fused_chunks). An nvfp4 row's maximum
 // goes through the cluster's shared memory: each CTA posts its slice's.
 #include "fp4_common.cuh"
 #include "gemm_internal.h"
@@ -64,8 +64,9 @@ struct Cfg {
 __host__ __device__ __forceinline__ int column_share(int mcols, int S) { return ((mcols + S - 1) / S + 3) & ~3; }
 
 // Chunks of eight values that a thread of FUSED takes at most. Measured against the two
-// kernels at M = 1: 4096 x 12288 mxfp4 10.7 / 15.0 us, nvfp4 14.0 / 18.4 (2 chunks); 24576 x
-// 4096 mxfp4 14.9 / 14.6, nvfp4, which reads twice through its maxima, 19.1 / 17.4 (4 chunks).
+// kernels at M = 1, in a graph: 4096 x 12288 mxfp4 10.3 / 11.9 us, nvfp4 12.7 / 13.7; 6144 x 4096
+// mxfp4 7.3 / 7.9, nvfp4 9.6 / 8.0 (called eagerly one launch less counts for more); 24576 x 4096
+// mxfp4 14.7 / 14.8 (4 chunks); nvfp4, which reads twice through its maxima, lost 1.7 us there.
 __host__ __device__ constexpr int fused_chunks(int fmt) { return fmt == FNI8_MXFP4 ? 4 : 2; }
 
 // FUSED: the epilogue warps' part before the product. 128 threads; xs: nk stages of X_STAGE

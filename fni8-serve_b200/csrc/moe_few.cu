@@ -1,4 +1,5 @@
-// The routed-expert layer for a few tokens (T <= 16) in two kernels, or three:
+// The routed-expert layer for a few tokens (T <= 16, as long as the int8 rows of x and of every
+// slot's h fit into shared memory beside the rings) in two kernels, or three:
 //
 //   few_gate_up  logits -> top-k (optional), int8 rows of x, then per active expert e and slot
 //                (t, j) routed to it   h[slot] = T(T(act(g)) u),
@@ -751,10 +752,10 @@ int few_stages(int cols, int rows, int64_t k_len, int slots, int E, int extra) {
   return 0;
 }
 
-// CTAs per cluster that share the preparation. Four, where the rows have 16384 values in all:
-// 4 tokens of 8 large experts 59 us, 63 in pairs, 64 in clusters of eight, which leave 28 of the
-// 148 SMs idle; fewer values are sooner
-// quantised than shared (one token of 2048: 20.9 us, in clusters 21.1).
+// CTAs per cluster that share the preparation. Four, where the rows have 16384 values in all: 4
+// tokens of 8 large experts 59 us when this was chosen (56 now), 63 in pairs, 64 in clusters of eight,
+// which leave 28 of the 148 SMs idle; fewer values are sooner quantised than shared (one token of
+// 2048: 20.9 us, in clusters 21.1).
 int few_cluster(int64_t rows, int64_t k_len) { return rows * k_len >= 16384 ? 4 : 1; }
 
 // Grid of `want` CTAs at most, in clusters of cs that are resident at once.
