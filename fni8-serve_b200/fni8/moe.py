@@ -167,13 +167,19 @@ class ExpertStack:
         return ExpertStack(self.w_gu.to(device), self.s_gu.to(device), self.w_dn.to(device), self.s_dn.to(device))
 
 
+def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
+    """x as contiguous rows that start on a 16-byte boundary (the kernels' vector loads)."""
+    x = x.contiguous()
+    return x.clone() if x.data_ptr() & 15 else x
+
+
 def experts(x: torch.Tensor, topi: torch.Tensor, topw: torch.Tensor, stack: ExpertStack,
             act: str = "silu") -> torch.Tensor:
     """Routed-expert output for x[T, H] given the routing (one native call)."""
     _need_cuda(x, "moe.experts")
     if act not in _ACT:
         raise ValueError(f"unsupported activation {act!r}")
-    x2 = x.contiguous()
+    x2 = _aligned_rows(x)
     T, H = x2.shape
     k = topi.shape[1]
     E, I = stack.num_experts, stack.intermediate
@@ -207,7 +213,7 @@ def layer(x: torch.Tensor, logits: torch.Tensor, stack: ExpertStack, top_k: int,
     dev = x.device
     if logits.device != dev or stack.w_gu.device != dev:
         raise RuntimeError("fni8.moe.layer: x, logits and experts are on different devices")
-    x2 = x.contiguous()
+    x2 = _aligned_rows(x)
     lg = (logits if logits.dtype == torch.float32 else logits.float()).contiguous()
     T, H = x2.shape
     bias = None

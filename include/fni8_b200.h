@@ -373,9 +373,10 @@ FNI8_API int fni8_moe_experts_w8a8(const void* x, int dtype, int64_t T, int64_t 
 /* The same from the router's logits [T, E] on: fni8_moe_route (weights rounded to dtype), then
  * fni8_moe_experts_w8a8 (SparseMoE.forward without the shared expert,
  * fni8serve/models/moe.py:62-105); the routing is not returned. Up to 16 tokens, where the
- * int8 rows fit into shared memory (about T top_k (I + 150) and T H up to 160,000), run in two or three kernels that read each active expert's weights
- * once (fni8_moe_experts_w8a8 likewise); the results are those of the separate calls, bit for
- * bit, for any T. E <= 512. */
+ * int8 rows fit into shared memory (about T top_k (I + 150) and T H up to 160,000), run in two
+ * or three kernels that read each active expert's weights once (fni8_moe_experts_w8a8 likewise);
+ * the results are those of the separate calls, bit for bit, for any T. E <= 512, H and I a
+ * multiple of 16, x 16-byte aligned, workspace 256-byte aligned. */
 FNI8_API size_t fni8_moe_layer_workspace_bytes(int64_t T, int64_t H, int64_t top_k, int64_t E, int64_t I);
 FNI8_API int fni8_moe_layer_w8a8(const void* x, int dtype, int64_t T, int64_t H, const float* logits, int64_t top_k,
                                  int scoring, const float* sel_bias, int64_t n_groups, int64_t topk_group,

@@ -62,3 +62,21 @@ def test_formula_in_fp32(T, dtype):
         for j in range(k):
             out = out + topw[:, j:j + 1] * y[:, j]
         assert torch.equal(moe.layer(x, logits, stack, k), out.to(dtype))
+
+
+@pytest.mark.parametrize("T", [1, 4, 16, 40])
+@pytest.mark.parametrize("offset", [1, 2, 4])
+def test_rows_at_any_address(T, offset):
+    """x as a view into a flat buffer at an odd place: the values of its copy."""
+    from fni8 import moe
+
+    E, k, H, I = 8, 2, 128, 64
+    stack = make_stack(E, H, I, 2)
+    x, logits = inputs(T, E, H, torch.bfloat16, T)
+    flat = torch.empty(offset + T * H, dtype=x.dtype, device=DEV)
+    flat[offset:] = x.reshape(-1)
+    view = flat[offset:].view(T, H)
+    assert view.data_ptr() % 16
+    topi, topw = moe.route(logits, k, weight_dtype=x.dtype)
+    assert torch.equal(moe.layer(view, logits, stack, k), moe.layer(x, logits, stack, k))
+    assert torch.equal(moe.experts(view, topi, topw, stack), moe.experts(x, topi, topw, stack))
