@@ -536,14 +536,15 @@ __global__ void __launch_bounds__(kThreads) few_down(const __grid_constant__ CUt
   int n_ent;
   if (p.early) {
     for (int i = threadIdx.x; i < p.E * ((n + 31) >> 5); i += kThreads) reinterpret_cast<uint32_t*>(smem + pl.masks)[i] = 0u;
-    // The routing's inputs are older than few_gate_up, which released this kernel after its own
-    // wait for them: they are read before this kernel waits for few_gate_up.
+    // The routing's inputs (and the weights that the ring loads) are older than few_gate_up, which
+    // released this kernel after its own wait for them: what wrote them had ended, its stores were in
+    // L2. So they are read before this kernel waits for few_gate_up, and from L2.
     if (p.logits != nullptr) {
       for (int t = warp * peers + rank; t < p.T; t += kWarps * peers) route_one(p, t, lane, slot_e, slot_w, peers);
     } else {
       for (int i = threadIdx.x; i < n; i += kThreads) {
-        slot_e[i] = p.topi[i];
-        slot_w[i] = p.topw[i];
+        slot_e[i] = __ldcg(p.topi + i);
+        slot_w[i] = __ldcg(p.topw + i);
       }
     }
     join(peers);

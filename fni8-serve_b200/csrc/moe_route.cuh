@@ -31,7 +31,8 @@ __device__ __forceinline__ void warp_argmax(float& v, int& i) {
 }
 
 // Scores of logits row `lr` [E] and the top k of them: lane j < k returns slot j's expert in
-// `out_i` and its weight in `out_w`. VPL = experts per lane (E <= 32 * VPL).
+// `out_i` and its weight in `out_w`. VPL = experts per lane (E <= 32 * VPL). The inputs are read
+// from L2: few_down routes before its own wait, where a line of an older call in L1 may be stale.
 template <int VPL>
 __device__ __forceinline__ void route_token(const float* __restrict__ lr, int E, int k, int scoring,
                                             const float* __restrict__ sel_bias, int n_groups, int topk_group,
@@ -42,7 +43,7 @@ __device__ __forceinline__ void route_token(const float* __restrict__ lr, int E,
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
     const int e = lane + 32 * i;
-    sc[i] = e < E ? lr[e] : NEG;
+    sc[i] = e < E ? __ldcg(lr + e) : NEG;
   }
   if (scoring == FNI8_SCORE_SOFTMAX) {
     float mx = NEG;
@@ -67,7 +68,7 @@ __device__ __forceinline__ void route_token(const float* __restrict__ lr, int E,
     for (int i = 0; i < VPL; ++i) {
       const int e = lane + 32 * i;
       sc[i] = e < E ? __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-sc[i]))) : 0.0f;
-      sel[i] = e < E ? (sel_bias ? __fadd_rn(sc[i], sel_bias[e]) : sc[i]) : NEG;
+      sel[i] = e < E ? (sel_bias ? __fadd_rn(sc[i], __ldcg(sel_bias + e)) : sc[i]) : NEG;
     }
   }
   if (n_groups > 0 && topk_group > 0) {

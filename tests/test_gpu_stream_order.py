@@ -114,3 +114,51 @@ def test_clusters_of_two_streams(scheme):
     torch.cuda.synchronize()
     assert all(torch.equal(y, want[i]) for i, y in got)
     assert fni8.device_status() == 0
+
+
+@pytest.mark.parametrize("E,k,H,I", [(4, 1, 2048, 16), (16, 4, 512, 256), (64, 6, 1040, 208)])
+@pytest.mark.parametrize("T", [1, 3])
+def test_routing_and_experts_rewritten_in_place(T, E, k, H, I):
+    """The MoE layer directly behind the kernels that write its logits, bias, rows and weights, at the addresses that
+    the call before read: layers whose second kernel has more CTAs than the first, eager and in a graph."""
+    from fni8 import moe
+
+    g = torch.Generator(device=DEV).manual_seed(T)
+
+    def values():
+        def w(n, m):
+            return (torch.randint(-127, 128, (E, n, m), generator=g, device=DEV, dtype=torch.int8),
+                    (0.5 + torch.rand(E, n, generator=g, device=DEV)) * (2.0 / (127 * m ** 0.5)))
+
+        return (torch.randn(T, H, generator=g, device=DEV).half(), torch.randn(T, E, generator=g, device=DEV),
+                0.3 * torch.randn(E, generator=g, device=DEV), *w(2 * I, H), *w(H, I))
+
+    def call(v):
+        x, logits, bias, *w = v
+        return moe.layer(x, logits, moe.ExpertStack(*w), k, scoring="sigmoid", sel_bias=bias)
+
+    src = [values() for _ in range(4)]
+    live = [t.clone() for t in src[0]]
+    want = [call(v) for v in src]
+    torch.cuda.synchronize()
+
+    def rewrite(v, order):
+        for i in order:
+            live[i].copy_(v[i])
+
+    got, order = [], [0, 3, 1, 2, 3, 0, 2, 1]
+    for n, i in enumerate(order):  # the routing's inputs last, then the weights last
+        rewrite(src[i], (0, 3, 4, 5, 6, 2, 1) if n % 2 else (1, 2, 0, 6, 4, 3, 5))
+        got.append(call(live))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for y, i in zip(got, order))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ys = []
+        for i in (1, 2, 0):
+            rewrite(src[i], (0, 3, 4, 5, 6, 2, 1))
+            ys.append(call(live))
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, want[i]) for y, i in zip(ys, (1, 2, 0)))
