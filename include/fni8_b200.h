@@ -270,7 +270,8 @@ FNI8_API int fni8_dequantize_rows_fp4(const uint8_t* q, const uint8_t* sf, const
  * and the result to out_dtype (F16 or BF16; bias in out_dtype or NULL). K is cut into parts by
  * M, N and K, so the order of a row's fp32 sum depends on M: the same for every call of the same
  * sizes, but a row alone and in a batch may differ in the last bits. Operands are read behind
- * griddepcontrol.wait: the kernel in front may be the one that writes them. q rows 16-byte aligned. No workspace:
+ * griddepcontrol.wait: the kernel in front may be the one that writes them. q rows 16-byte
+ * aligned. No workspace:
  * concurrent calls are independent. */
 FNI8_API int fni8_gemm_fp4(const uint8_t* a, const uint8_t* a_sf, const float* a_row_scale, const uint8_t* w,
                            const uint8_t* w_sf, const float* w_row_scale, const void* bias, void* out, int out_dtype,
